@@ -339,6 +339,60 @@ int vx_weighted_combine(const void* outputs, int32_t dtype, int32_t n_out, const
 int vx_rmsnorm(const uint16_t* x, const uint16_t* gain, int32_t T, int32_t d,
                float eps, uint16_t* y, void* stream);
 
+/* ---- 8-bit rows, products grouped by expert, adapters ------------------ */
+
+/* Rows in 8 bits: e4m3 values q with one float32 scale a row, standing for
+ * q * scale; scale = max(max|v| / 448, 2^-126).  A row with a NaN has a NaN
+ * scale.  The reference serves bf16 activations over 4-bit banks only; these
+ * entry points serve the same layer over bf16 or 8-bit banks. */
+#define VX_DTYPE_E4M3 2
+
+/* RMSNorm of s = x + residual (residual NULL: of x): y = bf16(s *
+ * (1/sqrt(mean(s^2)+eps)) * gain), and the same unrounded values as 8-bit
+ * rows (q [T, d], scales [T]); y or q/scales may be NULL, not both.  s stays
+ * in float32 inside; residual_out [T, d] receives it rounded to the
+ * residual's type, VX_DTYPE_BF16 or VX_DTYPE_F32 (NULL exactly when residual
+ * is).  Rows of x and residual lie ldx / ldr elements apart; outputs are
+ * contiguous and overlap no input. */
+int vx_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* residual, int32_t residual_dtype,
+                   int64_t ldr, const uint16_t* gain, int64_t T, int32_t d, float eps,
+                   void* residual_out, uint16_t* y, uint8_t* q, float* scales, void* stream);
+
+/* silu(gate) * up in float32, as 8-bit rows q [rows, width], scales [rows]:
+ * what a grouped product over e4m3 banks reads next. */
+int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_t ldu, int64_t rows,
+                   int32_t width, uint8_t* q, float* scales, void* stream);
+
+/* Products grouped by expert: for expert e and its positions p in
+ * [offsets[e], offsets[e+1]) (device int32 [experts+1], as vx_permute writes
+ * them)
+ *   out[p, :] = x[r(p), :] . w[e]^T,   r(p) = rows[p] / slots, or p (rows NULL)
+ * with w [experts, N, K].  dtype VX_DTYPE_BF16, or VX_DTYPE_E4M3 with
+ * x_scales [x_rows] and w_scales [experts, N]: then out is multiplied by
+ * both.  Sums in float32, out bf16.  rows and slots fit vx_permute's order
+ * over T * slots routed ids: a position reads its token's row of x.
+ * Positions from offsets[experts] on are left as they were; a position whose
+ * row lies outside [0, x_rows) gets zeros; offsets are clamped to
+ * [0, P] and to ascend.  K and ldx are multiples of 16 bytes, x and w start
+ * on 16-byte boundaries. */
+int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx, const void* w,
+                      const float* x_scales, const float* w_scales, const int32_t* offsets,
+                      int32_t experts, int32_t N, int32_t K, const int32_t* rows, int32_t slots,
+                      int64_t P, uint16_t* out, int64_t ldo, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection whose output
+ * is y: out[t, :] = y[t, :] + scales[e] * b[e] (a[e] x[t, :]) with e =
+ * adapters[t] (device int32 [T]), a [L, R, K], b [L, N, R] bf16, of which the
+ * first ranks[e] (clamped to 0..R) of the R components count; scales and
+ * ranks may be NULL (1 and R).  A token whose adapter is outside [0, L) gets
+ * y.  Sums in float32, one rounding.  out may be y itself (ldo == ldy).  K
+ * and R are multiples of 8, R <= 256; x, a and b start on 16-byte
+ * boundaries, as do the rows of x. */
+int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a,
+                const uint16_t* b, const int32_t* adapters, const float* scales, const int32_t* ranks,
+                int32_t L, int64_t T, int32_t K, int32_t N, int32_t R, uint16_t* out, int64_t ldo,
+                void* stream);
+
 /* ---- Stage timing ----------------------------------------------------- */
 
 /* Per-kernel boundary timing, the role of the reference's BoundaryProfiler

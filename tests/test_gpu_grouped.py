@@ -1,0 +1,200 @@
+"""grouped_matmul against its definition in 64 bits: ragged groups from empty
+to several tiles, odd outputs, every kind of row order, strided operands,
+positions behind the last group, bad offsets and rows."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import vxmoe
+from rows64 import BF16, F32, grouped64, sum_tol, within
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(seed, *shape, spread=1.0):
+    return (torch.randn(shape, device="cuda", generator=gen(seed)) * spread).bfloat16()
+
+
+def operands(kind, M, E, N, K, seed=1):
+    """x, w and their scales (None for bf16)."""
+    x, w = normal(seed, M, K), normal(seed + 1, E, N, K, spread=0.05)
+    if kind == "bf16":
+        return x, w, None, None
+    xs = torch.rand(M, device="cuda", generator=gen(seed + 2)) + 0.5
+    ws = torch.rand((E, N), device="cuda", generator=gen(seed + 3)) * 0.02 + 0.01
+    return (x * 20).to(torch.float8_e4m3fn), (w * 400).to(torch.float8_e4m3fn), xs, ws
+
+
+def offsets_of(counts):
+    c = torch.tensor([0] + list(counts), device="cuda").cumsum(0)
+    return c.int()
+
+
+def check(x, w, offsets, what, **kw):
+    got = vxmoe.grouped_matmul(x, w, offsets, **kw)
+    kw.pop("out", None)
+    want, size = grouped64(x, w, offsets, **kw)
+    assert got.dtype == torch.bfloat16
+    within(got[:want.shape[0]], want, want.abs() * (BF16 + 8 * F32) + size * sum_tol(x.shape[1]), what)
+    return got
+
+
+COUNTS = [
+    [1], [0, 0, 3, 0], [16, 17, 31, 32, 33], [0, 255, 256, 257, 0, 1], [300, 5, 700], [1] * 40, [513, 0, 0, 2],
+]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("counts", COUNTS, ids=lambda c: "-".join(map(str, c[:8])))
+@pytest.mark.parametrize("N,K", [(96, 64), (257, 208), (300, 1024)])
+def test_sorted_rows(kind, counts, N, K):
+    P = sum(counts)
+    x, w, xs, ws = operands(kind, P, len(counts), N, K)
+    check(x, w, offsets_of(counts), f"{kind} {counts} {N}x{K}", x_scales=xs, w_scales=ws)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("N", [1, 2, 7, 8, 127, 128, 129, 255, 256, 511, 640])
+@pytest.mark.parametrize("K", [16, 48, 64, 80, 128])
+def test_odd_outputs_and_inputs(kind, N, K):
+    x, w, xs, ws = operands(kind, 45, 3, N, K)
+    check(x, w, offsets_of([20, 4, 21]), f"{kind} {N}x{K}", x_scales=xs, w_scales=ws)
+
+
+def routed(T, E, k, seed):
+    ids = torch.rand((T, E), device="cuda", generator=gen(seed)).topk(k, dim=1).indices.int()
+    return ids, vxmoe.permute(ids, E)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("T,E,k,N,K", [(1, 32, 10, 128, 256), (1, 1, 1, 65, 64), (64, 128, 10, 264, 512),
+                                       (300, 16, 4, 130, 144), (2000, 8, 2, 256, 64), (37, 512, 10, 32, 128)])
+def test_routed_rows(kind, T, E, k, N, K):
+    x, w, xs, ws = operands(kind, T, E, N, K, seed=5)
+    _, p = routed(T, E, k, 6)
+    check(x, w, p.offsets, f"{kind} T={T} E={E}", rows=p.order, slots=k, x_scales=xs, w_scales=ws)
+
+
+def test_rows_without_slots_and_the_same_row_often():
+    x, w, _, _ = operands("bf16", 9, 4, 72, 96)
+    rows = torch.tensor([8, 8, 8, 0, 1, 0, 5, 5, 2, 3], device="cuda", dtype=torch.int32)
+    check(x, w, offsets_of([3, 0, 5, 2]), "rows", rows=rows)
+    check(x, w, offsets_of([3, 0, 5, 2]), "rows as int64", rows=rows.long())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_positions_behind_the_last_group_are_left(kind, gather):
+    x, w, xs, ws = operands(kind, 50, 3, 40, 64)
+    rows = torch.randint(0, 50, (50,), device="cuda", generator=gen(7), dtype=torch.int32) if gather else None
+    out = torch.full((50, 40), 7.0, dtype=torch.bfloat16, device="cuda")
+    offsets = offsets_of([5, 0, 12])
+    got = check(x, w, offsets, f"{kind} {gather}", rows=rows, x_scales=xs, w_scales=ws, out=out)
+    assert got.data_ptr() == out.data_ptr() and bool((out[17:] == 7).all())
+    out.fill_(3.0)
+    vxmoe.grouped_matmul(x, w, torch.zeros(4, dtype=torch.int32, device="cuda"), rows=rows, x_scales=xs,
+                         w_scales=ws, out=out)
+    assert bool((out == 3).all())
+
+
+def test_offsets_and_rows_out_of_range():
+    """Offsets are clamped to [0, P] and to ascend; a row outside x gives zeros."""
+    x, w, _, _ = operands("bf16", 20, 4, 24, 64)
+    out = torch.full((20, 24), 5.0, dtype=torch.bfloat16, device="cuda")
+    bad = torch.tensor([-3, 6, 4, 1000, 30], dtype=torch.int32, device="cuda")
+    vxmoe.grouped_matmul(x, w, bad, out=out)
+    want, size = grouped64(x, w, torch.tensor([0, 6, 6, 20, 20]))
+    # expert 1 has the descending pair [6, 4): nothing; expert 2 goes on from 4
+    again, size2 = grouped64(x[4:], w[2:3], torch.tensor([0, 16]))
+    got = out.double()
+    tol = sum_tol(64)
+    for lo, hi, ref, sz in ((0, 4, want[:4], size[:4]), (6, 20, again[2:], size2[2:])):
+        within(got[lo:hi], ref, ref.abs() * (BF16 + 8 * F32) + sz * tol, f"{lo}:{hi}")
+    rows = torch.tensor([0, 99, -1, 3, 20, 2**31 - 1, -2**31], dtype=torch.int32, device="cuda")
+    for kind in ("bf16", "e4m3"):
+        x, w, xs, ws = operands(kind, 20, 1, 24, 64)
+        x.view(torch.uint8)[1] = 0xFF          # a row of NaN that no position names
+        got = vxmoe.grouped_matmul(x, w, offsets_of([7]), rows=rows, x_scales=xs, w_scales=ws)
+        assert not got[[1, 2, 4, 5, 6]].float().any()
+        assert got[[0, 3]].float().isfinite().all()
+
+
+def test_a_group_does_not_see_its_neighbours():
+    """NaN and infinities in one expert's rows or bank stay there."""
+    for kind in ("bf16", "e4m3"):
+        x, w, xs, ws = operands(kind, 60, 3, 80, 128)
+        clean = vxmoe.grouped_matmul(x, w, offsets_of([20, 7, 33]), x_scales=xs, w_scales=ws)
+        x2, w2 = x.clone(), w.clone()
+        x2.view(torch.uint8)[20:27] = 0xFF
+        w2.view(torch.uint8)[1] = 0xFF
+        got = vxmoe.grouped_matmul(x2, w2, offsets_of([20, 7, 33]), x_scales=xs, w_scales=ws)
+        keep = torch.ones(60, dtype=torch.bool, device="cuda")
+        keep[20:27] = False
+        assert got[20:27].float().isnan().all()
+        assert torch.equal(got[keep].view(torch.int16), clean[keep].view(torch.int16))
+
+
+def test_strided_operands():
+    x, w, _, _ = operands("bf16", 33, 2, 50, 128)
+    wide = normal(9, 33, 300)
+    offsets = offsets_of([20, 13])
+    out = torch.zeros((33, 90), dtype=torch.bfloat16, device="cuda")
+    for view, what in ((wide[:, 8:136], "aligned slice"), (wide[:, 3:131], "odd slice"),
+                       (wide[:1, :128].expand(33, 128), "one row repeated"),
+                       (normal(10, 128, 33).t(), "columns")):
+        check(view, w, offsets, what)
+    check(x, w, offsets, "rows of a wider out", out=out[:, 20:70])
+    assert not out[:, :20].any() and not out[:, 70:].any()
+    check(x, w, offsets, "odd out", out=out[:, 1:51])
+
+
+def test_nothing_to_do():
+    x, w, _, _ = operands("bf16", 0, 2, 50, 64)
+    assert vxmoe.grouped_matmul(x, w, offsets_of([0, 0])).shape == (0, 50)
+    x, w, _, _ = operands("bf16", 4, 2, 50, 64)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    assert vxmoe.grouped_matmul(x, w, offsets_of([0, 0]), rows=none).shape == (0, 50)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_results_do_not_depend_on_the_batch(kind):
+    """A row's products are the same bits alone and among others, call after call."""
+    x, w, xs, ws = operands(kind, 400, 2, 144, 320)
+    whole = vxmoe.grouped_matmul(x, w, offsets_of([390, 10]), x_scales=xs, w_scales=ws)
+    again = vxmoe.grouped_matmul(x, w, offsets_of([390, 10]), x_scales=xs, w_scales=ws)
+    assert torch.equal(whole, again)
+    for i in (0, 200, 389):
+        one = vxmoe.grouped_matmul(x[i:i + 1], w, offsets_of([1, 0]),
+                                   x_scales=None if xs is None else xs[i:i + 1], w_scales=ws)
+        assert torch.equal(one[0], whole[i])
+
+
+def test_two_streams_and_two_graphs_at_once():
+    x, w, _, _ = operands("bf16", 700, 16, 264, 512)
+    counts = offsets_of([44] * 12 + [0, 1, 170, 1])
+    want = vxmoe.grouped_matmul(x, w, counts)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(vxmoe.grouped_matmul(x, w, counts))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    eager = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            eager.append(vxmoe.grouped_matmul(x, w, counts))
+    torch.cuda.synchronize()
+    for got in outs + eager:
+        assert torch.equal(got, want)

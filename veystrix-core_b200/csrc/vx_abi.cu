@@ -1086,4 +1086,60 @@ int vx_rmsnorm(const uint16_t* x, const uint16_t* gain, int32_t T, int32_t d, fl
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 
+int vx_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* residual, int32_t residual_dtype, int64_t ldr,
+                   const uint16_t* gain, int64_t T, int32_t d, float eps, void* residual_out, uint16_t* y,
+                   uint8_t* q, float* scales, void* stream) {
+  if (T < 0 || T > 0x7FFFFFFF || d < 1 || ldx < 0 || ldr < 0) return VX_EINVAL_SHAPE;
+  if (residual && residual_dtype != VX_DTYPE_BF16 && residual_dtype != VX_DTYPE_F32) return VX_EINVAL_DTYPE;
+  if (T == 0) return VX_OK;   // empty tensors may come as null pointers
+  if ((q == nullptr) != (scales == nullptr) || (!y && !q) || (residual == nullptr) != (residual_out == nullptr))
+    return VX_EINVAL_SHAPE;
+  if (!x || !gain) return VX_EINVAL_SHAPE;
+  cudaError_t e = launch_add_rmsnorm(x, ldx, residual, residual_dtype == VX_DTYPE_F32, ldr, gain, T, d, eps,
+                                     residual_out, y, q, scales, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
+}
+
+int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_t ldu, int64_t rows, int32_t width,
+                   uint8_t* q, float* scales, void* stream) {
+  if (rows < 0 || rows > 0x7FFFFFFF || width < 1 || ldg < 0 || ldu < 0) return VX_EINVAL_SHAPE;
+  if (rows == 0) return VX_OK;
+  if (!gate || !up || !q || !scales) return VX_EINVAL_SHAPE;
+  cudaError_t e = launch_swiglu_e4m3(gate, ldg, up, ldu, rows, width, q, scales, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
+}
+
+int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx, const void* w,
+                      const float* x_scales, const float* w_scales, const int32_t* offsets, int32_t experts,
+                      int32_t N, int32_t K, const int32_t* rows, int32_t slots, int64_t P, uint16_t* out,
+                      int64_t ldo, void* stream) {
+  if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return VX_EINVAL_DTYPE;
+  const int size = dtype == VX_DTYPE_BF16 ? 2 : 1;
+  if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1) return VX_EINVAL_SHAPE;
+  if (P < 0 || P > 0x7FFFFFFF || x_rows < 0 || x_rows > 0x7FFFFFFF || ldo < N) return VX_EINVAL_SHAPE;
+  if (!rows && (x_rows < P || slots != 1)) return VX_EINVAL_SHAPE;
+  // rows and banks are read in pieces of 16 bytes
+  if (int64_t(K) * size % 16 || ldx < K || ldx * size % 16) return VX_EINVAL_SHAPE;
+  if (P == 0) return VX_OK;   // empty tensors may come as null pointers
+  if (dtype == VX_DTYPE_BF16 ? (x_scales || w_scales) : (!x_scales || !w_scales)) return VX_EINVAL_SHAPE;
+  if (!x || !w || !offsets || !out || x_rows < 1 || !aligned16(x) || !aligned16(w)) return VX_EINVAL_SHAPE;
+  GroupedArgs a{x, x_rows, ldx, w, x_scales, w_scales, offsets, experts, N, K, rows, slots, P, out, ldo};
+  cudaError_t e = launch_grouped(a, dtype == VX_DTYPE_E4M3, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
+}
+
+int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a, const uint16_t* b,
+                const int32_t* adapters, const float* scales, const int32_t* ranks, int32_t L, int64_t T, int32_t K,
+                int32_t N, int32_t R, uint16_t* out, int64_t ldo, void* stream) {
+  if (T < 0 || T > 0x7FFFFFFF || L < 1 || K < 8 || K % 8 || N < 1 || R < 8 || R % 8 || R > kLoraMaxRank)
+    return VX_EINVAL_SHAPE;
+  if (ldy < N || ldo < N || ldx < K || ldx % 8) return VX_EINVAL_SHAPE;
+  if (T == 0) return VX_OK;
+  if (!y || !x || !a || !b || !adapters || !out || !aligned16(x) || !aligned16(a) || !aligned16(b))
+    return VX_EINVAL_SHAPE;
+  LoraArgs args{y, ldy, x, ldx, a, b, adapters, scales, ranks, L, K, N, R, T, out, ldo};
+  cudaError_t e = launch_lora(args, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
+}
+
 }  // extern "C"

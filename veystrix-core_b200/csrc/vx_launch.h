@@ -346,6 +346,52 @@ cudaError_t launch_weighted_combine(const void* outputs, int n_out, const int32_
                                     cudaStream_t st);
 cudaError_t launch_rmsnorm(const uint16_t* x, const uint16_t* gain, int T, int d, float eps,
                            uint16_t* y, cudaStream_t st);
+// RMSNorm of x + residual (null: of x; bf16 or float32 rows, the sum written
+// to residual_out in the same type), rows to bf16 (y, may be null) and to
+// e4m3 with a float32 scale each (q and scales, both or neither).
+cudaError_t launch_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* residual, bool residual_f32, int64_t ldr,
+                               const uint16_t* gain, int64_t T, int d, float eps, void* residual_out, uint16_t* y,
+                               uint8_t* q, float* scales, cudaStream_t st);
+// silu(gate) * up in float32, rows to e4m3 with a float32 scale each.
+cudaError_t launch_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_t ldu, int64_t rows,
+                               int width, uint8_t* q, float* scales, cudaStream_t st);
+
+// Products grouped by expert over bf16 or e4m3 banks (vx_grouped.cu).
+constexpr int kGroupedMaxExperts = 4096;
+struct GroupedArgs {
+  const void* x;                // [x_rows][ldx]
+  int64_t x_rows, ldx;
+  const void* w;                // [experts][N][K]
+  const float* x_scales;        // [x_rows] or null
+  const float* w_scales;        // [experts][N] or null
+  const int32_t* offsets;       // [experts + 1]
+  int experts, N, K;
+  const int32_t* rows;          // position p reads x row rows[p] / slots (null: row p)
+  int slots;
+  int64_t P;
+  uint16_t* out;                // [P][ldo]
+  int64_t ldo;
+};
+cudaError_t launch_grouped(const GroupedArgs& a, bool e4m3, cudaStream_t st);
+
+// Low-rank adapters (vx_lora.cu).
+constexpr int kLoraMaxRank = 256;
+struct LoraArgs {
+  const uint16_t* y;            // [T][ldy]
+  int64_t ldy;
+  const uint16_t* x;            // [T][ldx]
+  int64_t ldx;
+  const uint16_t *a, *b;        // [L][R][K], [L][N][R]
+  const int32_t* adapters;      // [T]
+  const float* scales;          // [L] or null
+  const int32_t* ranks;         // [L] or null
+  int L, K, N, R;
+  int64_t T;
+  uint16_t* out;                // [T][ldo]
+  int64_t ldo;
+};
+cudaError_t launch_lora(const LoraArgs& a, cudaStream_t st);
+
 cudaError_t launch_swiglu(const uint16_t* g, const uint16_t* u, uint16_t* out, int64_t n,
                           cudaStream_t st);
 cudaError_t launch_dequant(const vx_q4& bank, int expert, float* out, cudaStream_t st);

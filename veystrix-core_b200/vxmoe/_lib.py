@@ -23,6 +23,7 @@ VX_EUNSUPPORTED = 7
 
 VX_DTYPE_BF16 = 0
 VX_DTYPE_F32 = 1
+VX_DTYPE_E4M3 = 2
 
 c_int32 = ctypes.c_int32
 c_int64 = ctypes.c_int64
@@ -126,6 +127,13 @@ SIGNATURES = {
     "vx_ep_combine": (ctypes.c_int, [ctypes.POINTER(VxEpComm), c_int32, P, P, P, P, P]),
     "vx_rmsnorm": (ctypes.c_int, [P, P, c_int32, c_int32, c_float, P, P]),
     "vx_weighted_combine": (ctypes.c_int, [P, c_int32, c_int32, P, P, c_int64, c_int32, c_int32, P, P, P]),
+    "vx_add_rmsnorm": (ctypes.c_int, [P, c_int64, P, c_int32, c_int64, P, c_int64, c_int32, c_float, P, P, P, P,
+                                      P]),
+    "vx_swiglu_e4m3": (ctypes.c_int, [P, c_int64, P, c_int64, c_int64, c_int32, P, P, P]),
+    "vx_grouped_matmul": (ctypes.c_int, [P, c_int32, c_int64, c_int64, P, P, P, P, c_int32, c_int32, c_int32, P,
+                                         c_int32, c_int64, P, c_int64, P]),
+    "vx_lora_add": (ctypes.c_int, [P, c_int64, P, c_int64, P, P, P, P, P, c_int32, c_int64, c_int32, c_int32,
+                                   c_int32, P, c_int64, P]),
     "vx_profile_enable": (ctypes.c_int, [ctypes.c_int]),
     "vx_profile_read": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_int,
                                        ctypes.POINTER(ctypes.c_double),

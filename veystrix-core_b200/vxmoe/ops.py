@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -755,3 +755,254 @@ def rms_norm(x: torch.Tensor, gain: torch.Tensor, eps: float = 1e-6) -> torch.Te
     _lib.check(_lib.load().vx_rmsnorm(x2.data_ptr(), gain.data_ptr(), int(x2.shape[0]), d,
                                        float(eps), y.data_ptr(), _stream(x.device)), "rms_norm")
     return y.reshape(x.shape)
+
+
+# --------------------------------------------------------------------------
+# 8-bit rows, products grouped by expert, adapters
+# --------------------------------------------------------------------------
+
+
+def _row_view(t: torch.Tensor, name: str, dtype: torch.dtype, align: int = 1):
+    """t as [rows, width] rows with unit stride inside a row, and their
+    stride: the tensor's own rows where they lie so (a slice of a wider
+    tensor), else a contiguous copy.  Rows start on `align`-byte boundaries."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on a CUDA device (no CPU path)")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
+    if t.dim() != 2:
+        if t.dim() < 1 or t.shape[-1] == 0:
+            raise ValueError(f"{name} must have shape [..., width], got {tuple(t.shape)}")
+        t = t.reshape(-1, t.shape[-1])
+    n, d = t.shape
+    if d == 0:
+        raise ValueError(f"{name} must have shape [..., width], got {tuple(t.shape)}")
+    ld = t.stride(0) if n > 1 else d
+    if (t.stride(1) != 1 and d > 1) or ld < d:
+        t, ld = t.contiguous(), d
+    if align > 1 and (t.data_ptr() % align or ld * t.element_size() % align):
+        t, ld = t.clone(memory_format=torch.contiguous_format), d
+    return t, ld
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, x on {dev}")
+
+
+def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple) -> Optional[torch.Tensor]:
+    """A contiguous tensor of exactly this type and shape (or None)."""
+    if t is None:
+        return None
+    _require_cuda(t, name)
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    return _i32(t, dev, name)
+
+
+def _call(dev: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) on dev's current stream, with dev current."""
+    if torch.cuda.current_device() == dev.index:
+        status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status:
+        _lib.check(status, what)
+
+
+class AddNorm(NamedTuple):
+    y: Optional[torch.Tensor]          # bf16, x's shape ("bf16", "both")
+    residual: Optional[torch.Tensor]   # x + residual in the residual's type
+    q: Optional[torch.Tensor]          # float8_e4m3fn, x's shape ("e4m3", "both")
+    scales: Optional[torch.Tensor]     # float32, x's shape without the width
+
+
+def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.Tensor, eps: float = 1e-6,
+                 output: str = "bf16") -> AddNorm:
+    """RMSNorm of ``x + residual`` with gain, in one pass over the rows.
+
+    x bf16 [..., d]; residual of the same shape, bf16 or float32, or None.
+    The norm sees the float32 sum before its rounding to the residual's
+    type.  ``output``: "bf16" (``y``), "e4m3" (``q`` with one float32 scale a
+    row, standing for ``q * scale``), or "both" of the same unrounded values.
+    Where ``rms_norm`` is followed by an 8-bit product this saves the
+    separate addition and quantisation passes."""
+    if output not in ("bf16", "e4m3", "both"):
+        raise ValueError(f"output must be 'bf16', 'e4m3' or 'both', got {output!r}")
+    x2, ldx = _row_view(x, "x", torch.bfloat16)
+    T, d = x2.shape
+    dev = x2.device
+    _same_device(dev, residual=residual, gain=gain)
+    if _bf16(gain, "gain").numel() != d:
+        raise ValueError("gain must have the hidden size")
+    gain = gain.contiguous()
+    shape = x.shape
+    res_out = r2 = None
+    ldr, res_type = 0, _lib.VX_DTYPE_BF16
+    if residual is not None:
+        if residual.dtype == torch.float32:
+            res_type = _lib.VX_DTYPE_F32
+        elif residual.dtype != torch.bfloat16:
+            raise TypeError(f"residual must be bfloat16 or float32, got {residual.dtype}")
+        if residual.shape != shape:
+            raise ValueError(f"residual shape {tuple(residual.shape)} != {tuple(shape)}")
+        r2, ldr = _row_view(residual, "residual", residual.dtype)
+        res_out = torch.empty(shape, dtype=residual.dtype, device=dev)
+    y = torch.empty(shape, dtype=torch.bfloat16, device=dev) if output != "e4m3" else None
+    q = scales = None
+    if output != "bf16":
+        q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    _call(dev, "add_rms_norm", _lib.load().vx_add_rmsnorm, x2.data_ptr(), ldx, _ptr(r2), res_type, ldr,
+          gain.data_ptr(), T, d, float(eps), _ptr(res_out), _ptr(y), _ptr(q), _ptr(scales))
+    return AddNorm(y, res_out, q, scales)
+
+
+class E4M3Rows(NamedTuple):
+    q: torch.Tensor        # float8_e4m3fn [..., width]
+    scales: torch.Tensor   # float32 [...]
+
+
+def swiglu_e4m3(gate: torch.Tensor, up: torch.Tensor) -> E4M3Rows:
+    """``silu(gate) * up`` in float32 as 8-bit rows with one scale each: the
+    input of the next grouped product over e4m3 banks.  gate and up are bf16
+    [..., width] of one shape; the two halves of one product's rows are read
+    where they lie."""
+    g2, ldg = _row_view(gate, "gate", torch.bfloat16)
+    u2, ldu = _row_view(up, "up", torch.bfloat16)
+    if gate.shape != up.shape:
+        raise ValueError("gate and up must have the same shape")
+    dev = g2.device
+    _same_device(dev, up=u2)
+    rows, width = g2.shape
+    q = torch.empty(gate.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scales = torch.empty(gate.shape[:-1], dtype=torch.float32, device=dev)
+    _call(dev, "swiglu_e4m3", _lib.load().vx_swiglu_e4m3, g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width,
+          q.data_ptr(), scales.data_ptr())
+    return E4M3Rows(q, scales)
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: Optional[torch.Tensor] = None,
+                   slots: int = 1, x_scales: Optional[torch.Tensor] = None,
+                   w_scales: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Products grouped by expert over an unquantised or 8-bit bank.
+
+    Positions ``offsets[e] .. offsets[e+1]`` (int32 [E+1], ``permute``'s) are
+    multiplied by expert e's matrix: ``out[p] = x[r(p)] @ w[e].T`` with
+    ``r(p) = rows[p] // slots``, or p without ``rows``.  With ``rows`` and
+    ``slots`` = ``permute``'s order and the routed slots per token, every
+    position reads its token's row of x where it lies.  x [M, K] and w
+    [E, N, K] are bfloat16, or float8_e4m3fn with ``x_scales`` float32 [M] and
+    ``w_scales`` float32 [E, N] (one scale per row of x and of w).  Returns
+    bf16 [P, N], P the length of ``rows`` (or M); positions from
+    ``offsets[E]`` on are left as they were in ``out`` (undefined when it is
+    allocated here).  K must be a multiple of 16 bytes."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+        raise TypeError("x must be a bfloat16 or float8_e4m3fn tensor")
+    if x.dim() != 2:
+        raise ValueError(f"x must have shape [rows, K], got {tuple(x.shape)}")
+    x, ldx = _row_view(x, "x", x.dtype, align=16)
+    M, K = x.shape
+    dev = x.device
+    _require_cuda(w, "w")
+    if w.dtype != x.dtype:
+        raise TypeError(f"w must be {str(x.dtype)[6:]} as x, got {w.dtype}")
+    if w.dim() != 3 or w.shape[2] != K or 0 in w.shape or not w.is_contiguous():
+        raise ValueError(f"w must be a contiguous [experts, out, {K}], got {tuple(w.shape)}")
+    if w.data_ptr() % 16 or K * w.element_size() % 16:
+        raise ValueError("w must start on a 16-byte boundary and its rows be multiples of 16 bytes")
+    E, N = int(w.shape[0]), int(w.shape[1])
+    e4m3 = x.dtype == torch.float8_e4m3fn
+    if e4m3 != (x_scales is not None) or e4m3 != (w_scales is not None):
+        raise ValueError("float8_e4m3fn takes x_scales and w_scales, bfloat16 neither")
+    _same_device(dev, w=w, x_scales=x_scales, w_scales=w_scales, out=out)
+    x_scales = _vector(x_scales, "x_scales", torch.float32, (M,))
+    w_scales = _vector(w_scales, "w_scales", torch.float32, (E, N))
+    offsets = _ids(offsets, "offsets", dev)
+    if offsets.numel() != E + 1:
+        raise ValueError(f"offsets must hold {E + 1} values, got {offsets.numel()}")
+    P = M
+    if rows is not None:
+        rows = _ids(rows, "rows", dev).reshape(-1)
+        P = rows.numel()
+    elif slots != 1:
+        raise ValueError("slots needs rows")
+    if slots < 1:
+        raise ValueError("slots must be at least 1")
+    if out is None:
+        out = torch.empty((P, N), dtype=torch.bfloat16, device=dev)
+    else:
+        _require_cuda(out, "out")
+        if out.dtype != torch.bfloat16:
+            raise TypeError(f"out must be bfloat16, got {out.dtype}")
+        if tuple(out.shape) != (P, N) or (N > 1 and out.stride(1) != 1) or (P > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be rows of shape {(P, N)}, got {tuple(out.shape)}")
+    if P and not M:
+        raise ValueError("rows need rows of x")
+    _call(dev, "grouped_matmul", _lib.load().vx_grouped_matmul, x.data_ptr(),
+          _lib.VX_DTYPE_E4M3 if e4m3 else _lib.VX_DTYPE_BF16, M, ldx, w.data_ptr(), _ptr(x_scales), _ptr(w_scales),
+          offsets.data_ptr(), E, N, K, _ptr(rows), int(slots), P, out.data_ptr(),
+          out.stride(0) if P > 1 else N)
+    return out
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapters: torch.Tensor,
+             scales: Optional[torch.Tensor] = None, ranks: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside one shared projection.
+
+    ``y`` [..., N] bf16 is the projection's output for ``x`` [..., K] bf16
+    (``quantized_matmul(x, ...)``); token t of adapter e = ``adapters[t]``
+    gets ``y + scales[e] * b[e] @ (a[e] @ x)``, a token whose adapter is
+    outside [0, L) (-1: none) gets y.  a [L, R, K] and b [L, N, R] bf16;
+    ``scales`` float32 [L]; ``ranks`` int32 [L]: only the first ranks[e] of
+    the R components count.  ``out`` may be y itself.  K and R are multiples
+    of 8, R at most 256."""
+    x2, ldx = _row_view(x, "x", torch.bfloat16, align=16)
+    y2, ldy = _row_view(y, "y", torch.bfloat16)
+    T, K = x2.shape
+    N = y2.shape[1]
+    dev = x2.device
+    _require_cuda(a, "a")
+    _require_cuda(b, "b")
+    if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+        raise TypeError(f"a and b must be bfloat16, got {a.dtype} and {b.dtype}")
+    if a.dim() != 3 or 0 in a.shape or a.shape[2] != K or not a.is_contiguous():
+        raise ValueError(f"a must be a contiguous [adapters, rank, {K}], got {tuple(a.shape)}")
+    L, R = int(a.shape[0]), int(a.shape[1])
+    if tuple(b.shape) != (L, N, R) or not b.is_contiguous():
+        raise ValueError(f"b must be a contiguous {(L, N, R)}, got {tuple(b.shape)}")
+    if K % 8 or R % 8 or R > 256:
+        raise ValueError(f"K {K} and rank {R} must be multiples of 8, the rank at most 256")
+    if a.data_ptr() % 16 or b.data_ptr() % 16:
+        raise ValueError("a and b must start on 16-byte boundaries")
+    if x.shape[:-1] != y.shape[:-1]:
+        raise ValueError(f"x and y rows differ: {tuple(x.shape[:-1])} and {tuple(y.shape[:-1])}")
+    _same_device(dev, y=y2, a=a, b=b, scales=scales, ranks=ranks, out=out)
+    adapters = _ids(adapters, "adapters", dev)
+    if adapters.numel() != T:
+        raise ValueError(f"adapters must name one adapter a row ({T}), got {adapters.numel()}")
+    scales = _vector(scales, "scales", torch.float32, (L,))
+    ranks = _vector(ranks, "ranks", torch.int32, (L,))
+    if out is None:
+        out = torch.empty(y.shape, dtype=torch.bfloat16, device=dev)
+        ldo = N
+    else:
+        o2, ldo = _row_view(out, "out", torch.bfloat16)
+        if out.shape != y.shape or o2.data_ptr() != out.data_ptr():
+            raise ValueError(f"out must be rows of shape {tuple(y.shape)}, got {tuple(out.shape)}")
+    _call(dev, "lora_add", _lib.load().vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
+          b.data_ptr(), adapters.data_ptr(), _ptr(scales), _ptr(ranks), L, T, K, N, R, out.data_ptr(), ldo)
+    return out
