@@ -1116,7 +1116,8 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
   if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return VX_EINVAL_DTYPE;
   const int size = dtype == VX_DTYPE_BF16 ? 2 : 1;
   if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1) return VX_EINVAL_SHAPE;
-  if (P < 0 || P > 0x7FFFFFFF || x_rows < 0 || x_rows > 0x7FFFFFFF || ldo < N) return VX_EINVAL_SHAPE;
+  // position numbers, with a tile's padding, stay within 32 bits
+  if (P < 0 || P > 0x7FFF0000 || x_rows < 0 || x_rows > 0x7FFF0000 || ldo < N) return VX_EINVAL_SHAPE;
   if (!rows && (x_rows < P || slots != 1)) return VX_EINVAL_SHAPE;
   // rows and banks are read in pieces of 16 bytes
   if (int64_t(K) * size % 16 || ldx < K || ldx * size % 16) return VX_EINVAL_SHAPE;

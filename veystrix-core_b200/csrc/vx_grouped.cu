@@ -5,84 +5,434 @@
 // for the positions p in [offsets[e], offsets[e+1]) of expert e, row p =
 // rows[p] / slots, or p itself; the scales only with e4m3.  Sums in float32,
 // one rounding.  Positions from offsets[E] on are left as they were.
-#include <cuda_fp8.h>
+//
+// A CTA pair (cluster of two, cta_group::2) computes tiles of 256 outputs x
+// up to 256 positions of one expert with tcgen05.mma:
+//
+//   D[256 outputs][N positions] += W[256][K] . X[N][K]^T
+//
+// The bank's rows are the MMA's M side, so a group of any size fills it and
+// only N follows the ragged group (a multiple of 32): a group of one position
+// costs the bank's bytes and little else.  Each CTA of the pair stages its
+// own 128 bank rows and half of the positions, 128 bytes of K at a time
+// (64 bf16 or 128 e4m3 inputs), so a 256 x 256 tile moves 32 KB per CTA and
+// step through L2 where two single CTAs would move 48.  K past the end and
+// rows past a bank's outputs arrive as zeros.
+//
+// Warp roles of a CTA (384 threads):
+//   warp 0      TMA: its half of both operands into a ring of kStages stages;
+//               positions either as boxes of 16 consecutive rows or, with
+//               `rows`, four rows of x per gather4 copy (32 lanes, one copy
+//               each: 128 positions).  Both CTAs' copies complete on the
+//               leader's barrier.
+//   warp 1      leader only: one thread issues the MMAs of both CTAs and
+//               commits each stage back to both producers.
+//   warp 2      allocates TMEM: two accumulators of 256 columns, so that a
+//               tile's epilogue runs beside the next tile's MMAs.
+//   warps 4-11  epilogue: TMEM lane = output, column = position.
+// The grid is persistent (a pair per two SMs); pair i takes tiles i, i + G,
+// ...  Tiles are numbered expert by expert (prefix sums over the groups in
+// shared memory), so pairs running side by side share one bank and its
+// positions in L2.  A group of more than 256 positions is cut into equal
+// tiles rather than full ones and a rest.
+//
+// Every wait is bounded: one that runs out ends the CTA's roles, and the
+// tiles left over are filled with NaN.
+#include <cudaTypedefs.h>
 
+#include "vx_async.cuh"
 #include "vx_common.cuh"
 #include "vx_launch.h"
+#include "vx_tc.cuh"
 
 namespace vx {
 
-VX_DEVICE float elem_f32(const uint16_t* p) { return bf16_to_f32(__ldg(p)); }
-VX_DEVICE float elem_f32(const uint8_t* p) {
-  __nv_fp8_e4m3 v;
-  v.__x = __ldg(p);
-  return float(v);
-}
+constexpr int kGtRows = 256;                        // outputs of a pair's tile
+constexpr int kGtCols = 256;                        // positions of a tile, at most
+constexpr int kGtThreads = 384;
+constexpr int kGtStages = 6;
+constexpr int kGtHalf = 128 * 128;                  // 128 rows x 128 bytes of K
+constexpr int kGtStage = 2 * kGtHalf;               // bank rows, positions
+constexpr int kGtEpiWarps = 8;
+
+struct GroupedTc {
+  CUtensorMap tm_w, tm_x;
+  GroupedArgs a;
+  int row_tiles;                                    // 256-output tiles of a bank
+};
 
 // The row of x that position p reads; -1 where it lies outside x.
-VX_DEVICE int64_t row_of(const GroupedArgs& a, int64_t p) {
-  if (!a.rows) return p;
-  const int r = a.rows[p];
+VX_DEVICE int row_of(const GroupedArgs& a, int p) {
+  const int r = __ldg(a.rows + p);
   return r >= 0 && r / a.slots < a.x_rows ? r / a.slots : -1;
 }
 
-// One CTA = one expert x 64 outputs: 64 x 64 tiles, 4 x 4 outputs a thread,
-// 16 inputs of both operands at a time in shared memory.
-template <typename E>
-__global__ void __launch_bounds__(256) grouped_kernel(const GroupedArgs a) {
-  chain_begin();
-  __shared__ float xs[16][65], ws[16][65];
-  const E* x = static_cast<const E*>(a.x);
-  const E* w = static_cast<const E*>(a.w) + int64_t(blockIdx.x) * a.N * a.K;
-  const int64_t first = min(max(int64_t(a.offsets[blockIdx.x]), int64_t(0)), a.P);
-  const int64_t last = min(max(int64_t(a.offsets[blockIdx.x + 1]), first), a.P);
-  const int n0 = blockIdx.y * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int64_t p0 = first; p0 < last; p0 += 64) {
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += 16) {
-      for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-        const int r = i >> 4, k = i & 15;
-        float xv = 0.f, wv = 0.f;
-        if (p0 + r < last && k0 + k < a.K) {
-          const int64_t row = row_of(a, p0 + r);
-          if (row >= 0) xv = elem_f32(x + row * a.ldx + k0 + k);
-        }
-        if (n0 + r < a.N && k0 + k < a.K) wv = elem_f32(w + int64_t(n0 + r) * a.K + k0 + k);
-        xs[k][r] = xv;
-        ws[k][r] = wv;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xs[k][ty * 4 + i], ws[k][tx + 16 * j], acc[i][j]);
-      __syncthreads();
+VX_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Address of the same shared-memory location in CTA `rank` of the cluster.
+VX_DEVICE uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+VX_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+VX_DEVICE void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// TMA loads of a CTA pair: into the own shared memory, completing on a
+// barrier of either CTA (no multicast).
+VX_DEVICE void pair_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+VX_DEVICE void pair_load_2d(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+VX_DEVICE void pair_gather4(uint32_t dst, const void* map, int x, const int (&r)[4], uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+      : "memory");
+}
+
+// One MMA of the pair over 32 bytes of K (16 bf16 or 32 e4m3 inputs).
+template <bool FP8>
+VX_DEVICE void pair_mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool acc) {
+  if (FP8)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(int(acc))
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(int(acc))
+        : "memory");
+}
+// Arrives on `bar` of both CTAs once the MMAs issued so far are done.
+VX_DEVICE void pair_commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(uint16_t(3))
+      : "memory");
+}
+// float32 accumulator, both operands K-major, M = 256: bf16 (format 1) or
+// e4m3 (format 0 of kind::f8f6f4).
+template <bool FP8>
+VX_DEVICE uint32_t pair_idesc(int n) {
+  const uint32_t f = FP8 ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(kGtRows >> 4) << 24);
+}
+
+// Bounded wait of a role: false once this CTA has given up.
+VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
+  }
+  *dead = 1;
+  return false;
+}
+
+// A tile: expert, first output, first position and number of positions.
+struct Tile {
+  int e, row0, p0, n;
+};
+
+template <bool FP8, bool GATHER>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
+    grouped_kernel(const __grid_constant__ GroupedTc g) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t full[kGtStages], empty[kGtStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead, scan[kGtThreads / 32];
+  const GroupedArgs& a = g.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  // tiles before expert e, behind the ring
+  int* first_tile = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)) + kGtStages * kGtStage);
+
+  if (threadIdx.x == 0) {
+    dead = 0;
+    for (int s = 0; s < kGtStages; ++s) {
+      mbar_init_n(smem_u32(&full[s]), 1);
+      mbar_init_n(smem_u32(&empty[s]), 1);
     }
-    for (int i = 0; i < 4; ++i) {
-      const int64_t p = p0 + ty * 4 + i;
-      if (p >= last) continue;
-      float sx = 1.f;
-      if (a.x_scales) {
-        const int64_t row = row_of(a, p);
-        sx = row >= 0 ? a.x_scales[row] : 0.f;
+    for (int b = 0; b < 2; ++b) {
+      mbar_init_n(smem_u32(&acc_full[b]), 1);
+      mbar_init_n(smem_u32(&acc_empty[b]), 2 * kGtEpiWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  chain_wait();
+
+  // positions of expert e, clamped to [0, P] and to ascend
+  auto group = [&](int e, int* p) {
+    const int P = int(a.P);
+    const int lo = min(max(__ldg(a.offsets + e), 0), P);
+    *p = lo;
+    return min(max(__ldg(a.offsets + e + 1), lo), P) - lo;
+  };
+  // inclusive scan of the experts' tile counts, blockDim experts at a time
+  int carry = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += kGtThreads) {
+    const int e = e0 + threadIdx.x;
+    int p, v = 0;
+    if (e < a.experts) v = (group(e, &p) + kGtCols - 1) / kGtCols * g.row_tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) scan[warp] = v;
+    __syncthreads();
+    int before = carry, all = carry;
+    for (int w = 0; w < kGtThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      all += scan[w];
+    }
+    if (e < a.experts) first_tile[e + 1] = before + v;
+    carry = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first_tile[0] = 0;
+  const int tiles = carry;
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  auto tile_at = [&](int t) {
+    int lo = 0, hi = a.experts;   // the last e with first_tile[e] <= t
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (first_tile[m] <= t) lo = m; else hi = m;
+    }
+    const int i = t - first_tile[lo];
+    int p;
+    const int n = group(lo, &p), parts = (n + kGtCols - 1) / kGtCols;
+    const int part = i / g.row_tiles, rt = i - part * g.row_tiles;
+    const int each = ((n + parts - 1) / parts + 31) & ~31;
+    return Tile{lo, rt * kGtRows, p + part * each, min(each, n - part * each)};
+  };
+  const int steps = (a.K * (FP8 ? 1 : 2) + 127) >> 7;
+  auto stage_w = [&](int s) { return base + s * kGtStage; };
+  auto stage_x = [&](int s) { return base + s * kGtStage + kGtHalf; };
+
+  if (warp == 0) {
+    // ---- copies
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      const Tile c = tile_at(t);
+      const int half = ((c.n + 31) & ~31) >> 1;     // positions staged by each CTA
+      const int p0 = c.p0 + rank * half, w0 = c.row0 + rank * 128;
+      int r[4];
+      if (GATHER) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int p = p0 + 4 * lane + j;
+          r[j] = p < c.p0 + c.n ? max(row_of(a, p), 0) : 0;   // padding columns are not stored
+        }
       }
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + tx + 16 * j;
-        if (n >= a.N) continue;
-        const float sw = a.w_scales ? a.w_scales[int64_t(blockIdx.x) * a.N + n] : 1.f;
-        a.out[p * a.ldo + n] = f32_to_bf16(acc[i][j] * sx * sw);
+      for (int k = 0; k < steps; ++k) {
+        if (!role_wait(smem_u32(&empty[s]), ph, &dead)) {
+          ok = false;
+          break;
+        }
+        const uint32_t bar = in_cta(smem_u32(&full[s]), 0);
+        const int x = k * (FP8 ? 128 : 64);
+        if (lane == 0) {
+          if (rank == 0) mbar_expect(smem_u32(&full[s]), uint32_t(2 * kGtHalf + 2 * half * 128));
+          pair_load_3d(stage_w(s), &g.tm_w, x, w0, c.e, bar);
+        }
+        if (GATHER) {
+          if (4 * lane < half) pair_gather4(stage_x(s) + lane * 512, &g.tm_x, x, r, bar);
+        } else {
+          if (16 * lane < half) pair_load_2d(stage_x(s) + lane * 2048, &g.tm_x, x, p0 + 16 * lane, bar);
+        }
+        if (++s == kGtStages) s = 0, ph ^= 1;
       }
+    }
+    if (dead && rank == 0 && lane == 0) {
+      // given up: let the copies in flight land (bounded)
+      const uint64_t t0 = global_ns();
+      for (int i = 0; i < kGtStages; ++i)
+        while (!mbar_try(smem_u32(&full[i]), i < s ? ph ^ 1 : ph) && global_ns() - t0 < kWaitLimitNs) {
+        }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ---- MMAs of the pair
+    if (lane == 0) {
+      int s = 0, b = 0;
+      uint32_t ph = 0, aph = 1;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        const Tile c = tile_at(t);
+        const uint32_t idesc = pair_idesc<FP8>((c.n + 31) & ~31), d = tmem + b * kGtCols;
+        if (!role_wait(smem_u32(&acc_empty[b]), aph, &dead)) break;
+        tc_fence_after();
+        for (int k = 0; k < steps; ++k) {
+          if (!role_wait(smem_u32(&full[s]), ph, &dead)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t ad = sw128_desc(stage_w(s)), bd = sw128_desc(stage_x(s));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pair_mma<FP8>(d, ad + 2 * i, bd + 2 * i, idesc, k > 0 || i > 0);
+          pair_commit(smem_u32(&empty[s]));
+          if (++s == kGtStages) s = 0, ph ^= 1;
+        }
+        if (!ok) break;
+        pair_commit(smem_u32(&acc_full[b]));
+        if (++b == 2) b = 0, aph ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue
+    const int quarter = warp & 3, h = (warp - 4) >> 2;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    int b = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles; t += pairs) {
+      const Tile c = tile_at(t);
+      const int n = c.row0 + int(rank) * 128 + quarter * 32 + lane;   // this lane's output
+      float sw = 1.f;
+      if (FP8 && n < a.N) sw = __ldg(a.w_scales + int64_t(c.e) * a.N + n);
+      // factor of the column this lane looks up, for each chunk of 32 columns
+      float f[kGtCols / 64];
+      uint32_t real[kGtCols / 64];
+      if (FP8 || GATHER) {
+#pragma unroll
+        for (int i = 0; i < kGtCols / 64; ++i) {
+          const int col = (2 * i + h) * 32 + lane, p = c.p0 + col;
+          int row = -1;
+          if (col < c.n) row = GATHER ? row_of(a, p) : p;
+          f[i] = FP8 && row >= 0 ? __ldg(a.x_scales + row) : 1.f;
+          real[i] = __ballot_sync(0xFFFFFFFFu, row >= 0);
+        }
+      }
+      if (ok) ok = role_wait(smem_u32(&acc_full[b]), ph, &dead);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < kGtCols / 64; ++i) {
+        const int c0 = (2 * i + h) * 32;
+        if (c0 >= c.n) break;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (c0 + 16 * q >= c.n) break;
+          float v[16];
+          tmem_ld16(tmem + lanes + b * kGtCols + c0 + 16 * q, v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int col = c0 + 16 * q + j;
+            float o = v[j];
+            if (FP8) o *= __shfl_sync(0xFFFFFFFFu, f[i], 16 * q + j) * sw;
+            if (GATHER && !((real[i] >> (16 * q + j)) & 1u)) o = 0.f;
+            if (!ok) o = __uint_as_float(0x7FC00000u);
+            if (col < c.n && n < a.N) a.out[int64_t(c.p0 + col) * a.ldo + n] = f32_to_bf16(o);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(in_cta(smem_u32(&acc_empty[b]), 0));
+      if (++b == 2) b = 0, ph ^= 1;
     }
   }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the peer's copies and MMAs touch this CTA no more
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ---- host side --------------------------------------------------------------
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn_grouped() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p) : nullptr;
+  }();
+  return fn;
+}
+
+// 128 bytes of K (128-byte swizzle) x `box_rows` rows of [outer][rows][K].
+static bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t rows, int64_t ld, int64_t outer,
+                          int box_rows) {
+  auto fn = encode_fn_grouped();
+  if (!fn) return false;
+  const int size = fp8 ? 1 : 2;
+  const cuuint64_t dims[3] = {cuuint64_t(K), cuuint64_t(rows), cuuint64_t(outer)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * size, cuuint64_t(ld) * size * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {cuuint32_t(128 / size), cuuint32_t(box_rows), 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return fn(m, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, outer ? 3 : 2,
+            const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, bool GATHER>
+static cudaError_t launch_grouped_as(const GroupedTc& g, int pairs, cudaStream_t st) {
+  auto k = grouped_kernel<FP8, GATHER>;
+  const int smem = kGtStages * kGtStage + 1024 + (g.a.experts + 1) * int(sizeof(int));
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       kGtStages * kGtStage + 1024 + (kGroupedMaxExperts + 1) * int(sizeof(int)));
+  if (e != cudaSuccess) return e;
+  return launch_chained(k, dim3(2 * pairs), dim3(kGtThreads), size_t(smem), st, g);
 }
 
 cudaError_t launch_grouped(const GroupedArgs& a, bool e4m3, cudaStream_t st) {
   if (a.P == 0 || a.N == 0) return cudaSuccess;
-  const dim3 grid(unsigned(a.experts), unsigned((a.N + 63) / 64));
-  return e4m3 ? launch_chained(grouped_kernel<uint8_t>, grid, dim3(256), 0, st, a)
-              : launch_chained(grouped_kernel<uint16_t>, grid, dim3(256), 0, st, a);
+  GroupedTc g;
+  g.a = a;
+  g.row_tiles = (a.N + kGtRows - 1) / kGtRows;
+  if (!encode_k_rows(&g.tm_w, a.w, e4m3, a.K, a.N, a.K, a.experts, 128) ||
+      !encode_k_rows(&g.tm_x, a.x, e4m3, a.K, a.x_rows, a.ldx, 0, a.rows ? 1 : 16))
+    return cudaErrorInvalidValue;
+  // no more pairs than the groups can have tiles
+  const int64_t groups = (a.P + kGtCols - 1) / kGtCols + (a.P < a.experts ? a.P : a.experts);
+  if (groups * g.row_tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  int64_t pairs = sm_count() / 2;
+  if (groups * g.row_tiles < pairs) pairs = groups * g.row_tiles;
+  const int n = int(pairs);
+  if (e4m3) return a.rows ? launch_grouped_as<true, true>(g, n, st) : launch_grouped_as<true, false>(g, n, st);
+  return a.rows ? launch_grouped_as<false, true>(g, n, st) : launch_grouped_as<false, false>(g, n, st);
 }
 
 }  // namespace vx
