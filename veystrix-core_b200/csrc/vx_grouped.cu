@@ -20,16 +20,23 @@
 // rows past a bank's outputs arrive as zeros.
 //
 // Warp roles of a CTA (384 threads):
-//   warp 0      TMA: its half of both operands into a ring of kStages stages;
-//               positions either as boxes of 16 consecutive rows or, with
-//               `rows`, four rows of x per gather4 copy (32 lanes, one copy
-//               each: 128 positions).  Both CTAs' copies complete on the
+//   warp 0      TMA: the bank rows and, without `rows`, the positions (boxes
+//               of 128, 64, 32 and 16 rows that add up to them) into a ring
+//               of kGtStages stages.  Both CTAs' copies complete on the
 //               leader's barrier.
 //   warp 1      leader only: one thread issues the MMAs of both CTAs and
 //               commits each stage back to both producers.
-//   warp 2      allocates TMEM: two accumulators of 256 columns, so that a
-//               tile's epilogue runs beside the next tile's MMAs.
+//   warps 2, 3  with `rows`: gather4 copies, four rows of x each.  One thread
+//               a warp issues them with its row numbers from shared memory:
+//               the copy takes its operands in uniform registers, and 32
+//               lanes that issue one each are served one after the other
+//               (about 75 cycles a copy, 2,400 for the 128 rows of a stage
+//               whose MMAs take 512).  Warp 2 also allocates TMEM: two
+//               accumulators of 256 columns, so that a tile's epilogue runs
+//               beside the next tile's MMAs.
 //   warps 4-11  epilogue: TMEM lane = output, column = position.
+// Only rows of real positions are copied; the columns of a tile's padding
+// hold what the ring held before and are not stored.
 // The grid is persistent (a pair per two SMs); pair i takes tiles i, i + G,
 // ...  Tiles are numbered expert by expert (prefix sums over the groups in
 // shared memory), so pairs running side by side share one bank and its
@@ -56,7 +63,7 @@ constexpr int kGtStage = 2 * kGtHalf;               // bank rows, positions
 constexpr int kGtEpiWarps = 8;
 
 struct GroupedTc {
-  CUtensorMap tm_w, tm_x;
+  CUtensorMap tm_w, tm_x[4];                        // x: boxes of 16, 32, 64 and 128 rows (with `rows`: of one)
   GroupedArgs a;
   int row_tiles;                                    // 256-output tiles of a bank
 };
@@ -101,11 +108,11 @@ VX_DEVICE void pair_load_2d(uint32_t dst, const void* map, int x, int y, uint32_
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-VX_DEVICE void pair_gather4(uint32_t dst, const void* map, int x, const int (&r)[4], uint32_t bar) {
+VX_DEVICE void pair_gather4(uint32_t dst, const void* map, int x, int4 r, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
       "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
       : "memory");
 }
 
@@ -140,12 +147,22 @@ VX_DEVICE uint32_t pair_idesc(int n) {
   return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(kGtRows >> 4) << 24);
 }
 
+// mbar_try that also acquires what the other CTA of the pair released.
+VX_DEVICE bool pair_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait of a role: false once this CTA has given up.
 VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (mbar_try(bar, parity)) return true;
+  if (pair_try(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    if (mbar_try(bar, parity)) return true;
+    if (pair_try(bar, parity)) return true;
     if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
   }
   *dead = 1;
@@ -162,6 +179,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedTc g) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kGtStages], empty[kGtStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(16) int4 row_of_4[2][kGtCols / 2 / 8];   // warps 2, 3: rows of each copy
   __shared__ uint32_t tmem_slot;
   __shared__ int dead, scan[kGtThreads / 32];
   const GroupedArgs& a = g.a;
@@ -251,16 +269,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
       const Tile c = tile_at(t);
-      const int half = ((c.n + 31) & ~31) >> 1;     // positions staged by each CTA
+      const int half = ((c.n + 31) & ~31) >> 1;     // columns of each CTA
       const int p0 = c.p0 + rank * half, w0 = c.row0 + rank * 128;
-      int r[4];
-      if (GATHER) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int p = p0 + 4 * lane + j;
-          r[j] = p < c.p0 + c.n ? max(row_of(a, p), 0) : 0;   // padding columns are not stored
-        }
-      }
+      // rows copied by each CTA: its real positions, rounded up to the copies' size
+      constexpr int kUnit = GATHER ? 4 : 16;
+      auto copied = [&](int r) { return (min(max(c.n - r * half, 0), half) + kUnit - 1) & ~(kUnit - 1); };
+      const int mine = copied(rank);
+      const uint32_t bytes = 2 * kGtHalf + (copied(0) + copied(1)) * 128;
+      // lane i < 4 copies the box of 16 << i rows if `mine` has that bit; the
+      // larger boxes come first, so box i starts at the bits above it
+      const bool box = !GATHER && lane < 4 && ((mine >> (4 + lane)) & 1);
+      const int at = mine & ~((32 << lane) - 1);
       for (int k = 0; k < steps; ++k) {
         if (!role_wait(smem_u32(&empty[s]), ph, &dead)) {
           ok = false;
@@ -269,14 +288,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         const uint32_t bar = in_cta(smem_u32(&full[s]), 0);
         const int x = k * (FP8 ? 128 : 64);
         if (lane == 0) {
-          if (rank == 0) mbar_expect(smem_u32(&full[s]), uint32_t(2 * kGtHalf + 2 * half * 128));
+          if (rank == 0) mbar_expect(smem_u32(&full[s]), bytes);
           pair_load_3d(stage_w(s), &g.tm_w, x, w0, c.e, bar);
         }
-        if (GATHER) {
-          if (4 * lane < half) pair_gather4(stage_x(s) + lane * 512, &g.tm_x, x, r, bar);
-        } else {
-          if (16 * lane < half) pair_load_2d(stage_x(s) + lane * 2048, &g.tm_x, x, p0 + 16 * lane, bar);
-        }
+        if (box) pair_load_2d(stage_x(s) + at * 128, &g.tm_x[lane], x, p0 + at, bar);
         if (++s == kGtStages) s = 0, ph ^= 1;
       }
     }
@@ -315,6 +330,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         if (++b == 2) b = 0, aph ^= 1;
       }
     }
+  } else if (GATHER && (warp == 2 || warp == 3)) {
+    // ---- rows of x: this warp's copies are 0, 2, ... or 1, 3, ... of a stage
+    const int w = warp - 2;
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      const Tile c = tile_at(t);
+      const int half = ((c.n + 31) & ~31) >> 1;
+      const int p0 = c.p0 + rank * half, mine = min(max(c.n - int(rank) * half, 0), half);
+      const int copies = ((mine + 3) / 4 - w + 1) / 2;
+      __syncwarp();
+      if (lane < 16) {
+        int r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int q = 4 * (2 * lane + w) + j;
+          r[j] = q < mine ? max(row_of(a, p0 + q), 0) : 0;   // those columns are zeroed or not stored
+        }
+        row_of_4[w][lane] = make_int4(r[0], r[1], r[2], r[3]);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        for (int k = 0; k < steps; ++k) {
+          ok = role_wait(smem_u32(&empty[s]), ph, &dead);
+          if (!ok) break;
+          const uint32_t bar = in_cta(smem_u32(&full[s]), 0), dst = stage_x(s) + w * 512;
+#pragma unroll 4
+          for (int j = 0; j < copies; ++j)
+            pair_gather4(dst + j * 1024, &g.tm_x[0], k * (FP8 ? 128 : 64), row_of_4[w][j], bar);
+          if (++s == kGtStages) s = 0, ph ^= 1;
+        }
+      }
+      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+    }
   } else if (warp >= 4) {
     // ---- epilogue
     const int quarter = warp & 3, h = (warp - 4) >> 2;
@@ -329,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
       if (FP8 && n < a.N) sw = __ldg(a.w_scales + int64_t(c.e) * a.N + n);
       // factor of the column this lane looks up, for each chunk of 32 columns
       float f[kGtCols / 64];
-      uint32_t real[kGtCols / 64];
+      uint32_t real[kGtCols / 64];   // columns whose row lies inside x
       if (FP8 || GATHER) {
 #pragma unroll
         for (int i = 0; i < kGtCols / 64; ++i) {
@@ -422,9 +472,10 @@ cudaError_t launch_grouped(const GroupedArgs& a, bool e4m3, cudaStream_t st) {
   GroupedTc g;
   g.a = a;
   g.row_tiles = (a.N + kGtRows - 1) / kGtRows;
-  if (!encode_k_rows(&g.tm_w, a.w, e4m3, a.K, a.N, a.K, a.experts, 128) ||
-      !encode_k_rows(&g.tm_x, a.x, e4m3, a.K, a.x_rows, a.ldx, 0, a.rows ? 1 : 16))
-    return cudaErrorInvalidValue;
+  if (!encode_k_rows(&g.tm_w, a.w, e4m3, a.K, a.N, a.K, a.experts, 128)) return cudaErrorInvalidValue;
+  for (int i = 0; i < (a.rows ? 1 : 4); ++i)
+    if (!encode_k_rows(&g.tm_x[i], a.x, e4m3, a.K, a.x_rows, a.ldx, 0, a.rows ? 1 : 16 << i))
+      return cudaErrorInvalidValue;
   // no more pairs than the groups can have tiles
   const int64_t groups = (a.P + kGtCols - 1) / kGtCols + (a.P < a.experts ? a.P : a.experts);
   if (groups * g.row_tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
