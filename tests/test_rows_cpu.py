@@ -67,14 +67,20 @@ def test_grouped_matmul_refusals(lib):
 def test_lora_add_refusals(lib):
     from vxmoe import _lib
 
-    def call(y=P16, ldy=24, x=P16, ldx=64, a=P16, b=P16, ids=P16, L=2, T=3, K=64, N=24, R=8, out=P16, ldo=24):
-        return lib.vx_lora_add(y, ldy, x, ldx, a, b, ids, None, None, L, T, K, N, R, out, ldo, None)
+    def call(y=P16, ldy=24, x=P16, ldx=64, a=P16, b=P16, ids=P16, L=2, T=3, K=64, N=24, R=8, out=P16, ldo=24, ws=None,
+             nbytes=0):
+        return lib.vx_lora_add(y, ldy, x, ldx, a, b, ids, None, None, L, T, K, N, R, out, ldo, ws, nbytes, None)
 
-    for kw in (dict(T=-1), dict(T=1 << 31), dict(L=0), dict(K=0), dict(K=60), dict(N=0), dict(R=0), dict(R=12),
+    for kw in (dict(T=-1), dict(T=1 << 31), dict(L=0), dict(L=4097), dict(K=0), dict(K=60), dict(N=0), dict(R=0), dict(R=12),
                dict(R=264), dict(ldy=23), dict(ldo=23), dict(ldx=63), dict(ldx=68), dict(y=None), dict(x=None),
                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(x=ODD), dict(a=ODD), dict(b=ODD)):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw
     assert call(T=0, x=None, y=None, out=None) == _lib.VX_OK
+    need = lib.vx_lora_add_workspace(300, 2)
+    assert lib.vx_lora_add_workspace(256, 2) == 0 and need >= 2 * 300 * 4
+    for kw in (dict(), dict(ws=P16, nbytes=need - 1), dict(ws=ODD, nbytes=need)):
+        assert call(T=300, **kw) == _lib.VX_EWORKSPACE, kw
+    assert lib.vx_lora_add_workspace(-1, 2) == lib.vx_lora_add_workspace(1, 0) == 0
 
 
 def test_python_layer_takes_cuda_tensors_only():

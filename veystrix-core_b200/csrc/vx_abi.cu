@@ -1129,17 +1129,26 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 
+size_t vx_lora_add_workspace(int64_t T, int32_t L) {
+  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters) return 0;
+  return size_t(lora_workspace_bytes(T, L));
+}
+
 int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a, const uint16_t* b,
                 const int32_t* adapters, const float* scales, const int32_t* ranks, int32_t L, int64_t T, int32_t K,
-                int32_t N, int32_t R, uint16_t* out, int64_t ldo, void* stream) {
-  if (T < 0 || T > 0x7FFFFFFF || L < 1 || K < 8 || K % 8 || N < 1 || R < 8 || R % 8 || R > kLoraMaxRank)
+                int32_t N, int32_t R, uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                void* stream) {
+  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || K < 8 || K % 8 || N < 1 || R < 8 || R % 8 || R > kLoraMaxRank)
     return VX_EINVAL_SHAPE;
   if (ldy < N || ldo < N || ldx < K || ldx % 8) return VX_EINVAL_SHAPE;
   if (T == 0) return VX_OK;
   if (!y || !x || !a || !b || !adapters || !out || !aligned16(x) || !aligned16(a) || !aligned16(b))
     return VX_EINVAL_SHAPE;
   LoraArgs args{y, ldy, x, ldx, a, b, adapters, scales, ranks, L, K, N, R, T, out, ldo};
-  cudaError_t e = launch_lora(args, static_cast<cudaStream_t>(stream));
+  const size_t need = vx_lora_add_workspace(T, L);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4))
+    return VX_EWORKSPACE;
+  cudaError_t e = launch_lora(args, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 

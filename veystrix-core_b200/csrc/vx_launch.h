@@ -376,6 +376,7 @@ cudaError_t launch_grouped(const GroupedArgs& a, bool e4m3, cudaStream_t st);
 
 // Low-rank adapters (vx_lora.cu).
 constexpr int kLoraMaxRank = 256;
+constexpr int kLoraMaxAdapters = 4096;
 struct LoraArgs {
   const uint16_t* y;            // [T][ldy]
   int64_t ldy;
@@ -390,7 +391,8 @@ struct LoraArgs {
   uint16_t* out;                // [T][ldo]
   int64_t ldo;
 };
-cudaError_t launch_lora(const LoraArgs& a, cudaStream_t st);
+int64_t lora_workspace_bytes(int64_t T, int L);   // 0 for the batches that group themselves
+cudaError_t launch_lora(const LoraArgs& a, void* workspace, cudaStream_t st);
 
 cudaError_t launch_swiglu(const uint16_t* g, const uint16_t* u, uint16_t* out, int64_t n,
                           cudaStream_t st);

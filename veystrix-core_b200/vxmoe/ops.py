@@ -984,8 +984,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     L, R = int(a.shape[0]), int(a.shape[1])
     if tuple(b.shape) != (L, N, R) or not b.is_contiguous():
         raise ValueError(f"b must be a contiguous {(L, N, R)}, got {tuple(b.shape)}")
-    if K % 8 or R % 8 or R > 256:
-        raise ValueError(f"K {K} and rank {R} must be multiples of 8, the rank at most 256")
+    if K % 8 or R % 8 or R > 256 or L > 4096:
+        raise ValueError(f"K {K} and rank {R} must be multiples of 8, the rank at most 256, adapters ({L}) 4096")
     if a.data_ptr() % 16 or b.data_ptr() % 16:
         raise ValueError("a and b must start on 16-byte boundaries")
     if x.shape[:-1] != y.shape[:-1]:
@@ -1003,6 +1003,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         o2, ldo = _row_view(out, "out", torch.bfloat16)
         if out.shape != y.shape or o2.data_ptr() != out.data_ptr():
             raise ValueError(f"out must be rows of shape {tuple(y.shape)}, got {tuple(out.shape)}")
-    _call(dev, "lora_add", _lib.load().vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
-          b.data_ptr(), adapters.data_ptr(), _ptr(scales), _ptr(ranks), L, T, K, N, R, out.data_ptr(), ldo)
+    lib = _lib.load()
+    nbytes = lib.vx_lora_add_workspace(T, L)
+    # its own allocation: a captured graph keeps it in its own pool
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, "lora_add", lib.vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
+          b.data_ptr(), adapters.data_ptr(), _ptr(scales), _ptr(ranks), L, T, K, N, R, out.data_ptr(), ldo, _ptr(ws),
+          nbytes)
     return out
