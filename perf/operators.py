@@ -19,12 +19,12 @@ TINY = 2.0 ** -126          # the smallest scale of a row: the smallest normal f
 
 
 def _vxmoe():
-    """The framework's package, which lies in a folder of the repository."""
-    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "veystrix-core_b200")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    import vxmoe
-    return vxmoe
+    """The framework's package, which lies in a folder of the repository; a program imports it once."""
+    if "vxmoe" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                        "veystrix-core_b200"))
+        import vxmoe  # noqa: F401
+    return sys.modules["vxmoe"]
 
 
 # ---- cases ------------------------------------------------------------------
