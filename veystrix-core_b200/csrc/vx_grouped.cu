@@ -461,8 +461,9 @@ template <bool FP8, bool GATHER>
 static cudaError_t launch_grouped_as(const GroupedTc& g, int pairs, cudaStream_t st) {
   auto k = grouped_kernel<FP8, GATHER>;
   const int smem = kGtStages * kGtStage + 1024 + (g.a.experts + 1) * int(sizeof(int));
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       kGtStages * kGtStage + 1024 + (kGroupedMaxExperts + 1) * int(sizeof(int)));
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k),
+                             kGtStages * kGtStage + 1024 + (kGroupedMaxExperts + 1) * int(sizeof(int)), done);
   if (e != cudaSuccess) return e;
   return launch_chained(k, dim3(2 * pairs), dim3(kGtThreads), size_t(smem), st, g);
 }

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "vxmoe.h"
 
 namespace vx {
@@ -46,6 +48,19 @@ template <typename... KArgs, typename... Args>
 inline cudaError_t launch_streaming(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                     cudaStream_t st, Args... args) {
   return launch_chained_as(true, kernel, grid, block, smem, st, args...);
+}
+
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per
+// device: `done` is the kernel's own static word, a bit per device.
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // Tokens per work item of the tensor-pipe GEMV (an expert's run is cut into

@@ -414,7 +414,8 @@ static cudaError_t launch_lora_as(const LoraArgs& a, const int32_t* order, const
   if (n * C > 0x7FFFFFFF) return cudaErrorInvalidValue;
   auto k = lora_kernel<MT, WIDE>;
   const int smem = lora_smem(MT, a.R);
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, lora_smem(MT, kLoraMaxRank));
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), lora_smem(MT, kLoraMaxRank), done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(n * C));

@@ -18,11 +18,11 @@
 // over the bit patterns of |v|, an order in which NaN is above infinity, so a
 // NaN anywhere makes the row's scale NaN as the formula does.
 //
-// A row belongs to one warp (four rows a CTA) while its elements fit one
-// warp's registers, else to one CTA.  V is the elements a load brings: 8
-// where every row starts on a 16-byte boundary and the width is a multiple
-// of 8, else 1.  Rows too wide for the registers of 1,024 threads are read
-// twice (LOOP).
+// Rows are dealt round robin to groups of threads, a warp (four groups a CTA)
+// or a CTA; a group has its next row's loads in flight while it reduces and
+// writes the present one.  V is the elements a load brings: 8 where every row
+// starts on a 16-byte boundary and the width is a multiple of 8, else 1.
+// Rows too wide for the registers of 1,024 threads are read twice (LOOP).
 #include <cuda_fp8.h>
 
 #include <type_traits>
@@ -54,39 +54,56 @@ VX_DEVICE uint32_t bf16x2(float lo, float hi) {
   return r;
 }
 
-// 1/(1 + exp(-g)) within a few float32 ulp: with e = exp(-|g|) <= 1 the
-// denominator stays in [1, 2], where the approximate division is exact to 2
-// ulp, and nothing overflows.
+// 1/(1 + exp(-g)): with e = exp(-|g|) <= 1 the denominator stays in [1, 2],
+// where the approximate division is good to 2 ulp, and nothing overflows;
+// the fast exponential is off by |g| 2^-24 of e.
 VX_DEVICE float sigmoid_f32(float g) {
-  const float e = expf(-fabsf(g));
+  const float e = __expf(-fabsf(g));
   return __fdividef(g < 0.f ? e : 1.0f, 1.0f + e);
 }
 
-template <int V>
-VX_DEVICE void load_row(const uint16_t* p, float (&f)[V]) {
-  if constexpr (V == 8) {
-    const uint4 v = ldg_nc(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// V elements of a row as they lie in memory, and as float32.
+template <int V, typename E>
+struct Raw {
+  static constexpr int kWords = V * int(sizeof(E)) / 16;
+  uint4 w[kWords];
+  VX_DEVICE void load(const E* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    for (int i = 0; i < kWords; ++i) w[i] = ldg_nc(reinterpret_cast<const uint4*>(p) + i);
+  }
+  VX_DEVICE void load_again(const E* p) {   // what every row reads: kept in L1
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  VX_DEVICE void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  VX_DEVICE void get(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (sizeof(E) == 2) {
+          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
+          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        } else {
+          f[4 * i + j] = __uint_as_float(u[j]);
+        }
+      }
     }
-  } else {
-    f[0] = bf16_to_f32(__ldg(p));
   }
-}
-template <int V>
-VX_DEVICE void load_row(const float* p, float (&f)[V]) {
-  if constexpr (V == 8) {
-    const uint4 a = ldg_nc(p), b = ldg_nc(p + 4);
-    f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z),
-    f[3] = __uint_as_float(a.w), f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y),
-    f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
-  } else {
-    f[0] = __ldg(p);
-  }
-}
+};
+template <typename E>
+struct Raw<1, E> {
+  E v;
+  VX_DEVICE void load(const E* p) { v = __ldg(p); }
+  VX_DEVICE void load_again(const E* p) { v = __ldg(p); }
+  VX_DEVICE void zero() { v = 0; }
+  VX_DEVICE void get(float (&f)[1]) const { f[0] = sizeof(E) == 2 ? bf16_to_f32(uint16_t(v)) : float(v); }
+};
+
 template <int V>
 VX_DEVICE void store_row(uint16_t* p, const float (&f)[V]) {
   if constexpr (V == 8)
@@ -114,216 +131,245 @@ VX_DEVICE void store_row(uint8_t* p, const float (&f)[V]) {
 }
 
 // Sum (SUM) and largest bit pattern over the threads of a row: its warp, or
-// the CTA (ONE_WARP false).  Every thread adds the warps' sums in the same order.
+// the CTA (ONE_WARP false).  Every thread adds the warps' sums in the same
+// order.  Successive calls alternate `turn` between two sets of shared
+// memory, so one barrier a call is enough.
 template <bool ONE_WARP, bool SUM>
-VX_DEVICE void row_reduce(float& sum, uint32_t& top) {
+VX_DEVICE void row_reduce(float& sum, uint32_t& top, int& turn) {
   if (SUM) sum = warp_sum<32>(sum);
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (ONE_WARP) return;
-  __shared__ float sums[32];
-  __shared__ uint32_t tops[32];
+  __shared__ float sums[2][32];
+  __shared__ uint32_t tops[2][32];
   const int warps = blockDim.x >> 5;
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum, tops[threadIdx.x >> 5] = top;
+  if ((threadIdx.x & 31) == 0) sums[turn][threadIdx.x >> 5] = sum, tops[turn][threadIdx.x >> 5] = top;
   __syncthreads();
   sum = 0.f, top = 0;
   for (int w = 0; w < warps; ++w) {
-    if (SUM) sum += sums[w];
-    top = max(top, tops[w]);
+    if (SUM) sum += sums[turn][w];
+    top = max(top, tops[turn][w]);
   }
+  turn ^= 1;
 }
 
-// The place of this thread's row and its stride in it: ONE_WARP puts four
-// rows into a CTA.  Returns the first element's index / V.
+// This thread's group of rows: the first row, the stride, and the thread's
+// place in the row and number of threads in it.
 template <bool ONE_WARP>
-VX_DEVICE int row_place(int64_t* row, int* lanes) {
-  if (ONE_WARP) {
-    *row = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    *lanes = 32;
-    return threadIdx.x & 31;
+struct Group {
+  int64_t row, stride;
+  int place, threads;
+  VX_DEVICE Group() {
+    if (ONE_WARP) {
+      row = int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+      stride = int64_t(gridDim.x) * (blockDim.x >> 5);
+      place = threadIdx.x & 31, threads = 32;
+    } else {
+      row = blockIdx.x, stride = gridDim.x;
+      place = threadIdx.x, threads = blockDim.x;
+    }
   }
-  *row = blockIdx.x;
-  *lanes = blockDim.x;
-  return threadIdx.x;
-}
+};
 
 template <int V, int NV, bool ONE_WARP, typename RES, bool LOOP>
-__global__ void __launch_bounds__(1024) add_rmsnorm_kernel(
+__global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
     const uint16_t* __restrict__ x, int64_t ldx, const RES* __restrict__ residual, int64_t ldr,
     const uint16_t* __restrict__ gain, int64_t T, int d, float eps, RES* __restrict__ residual_out,
     uint16_t* __restrict__ y, uint8_t* __restrict__ q, float* __restrict__ scales) {
   chain_begin();
-  int64_t t;
-  int lanes;
-  const int i0 = row_place<ONE_WARP>(&t, &lanes) * V, step = lanes * V;
-  if (ONE_WARP && t >= T) return;   // whole warps
-  const uint16_t* xr = x + t * ldx;
-  const RES* rr = residual ? residual + t * ldr : nullptr;
-
-  // s of this thread's elements; kept in registers unless LOOP
-  float s[NV][V], g[NV][V];
-  float sum = 0.f;
-  uint32_t top = 0;
-  auto load = [&](int i, float (&sv)[V], float (&gv)[V]) {
-    load_row<V>(xr + i, sv);
-    if (rr) {
+  const Group<ONE_WARP> grp;
+  const int i0 = grp.place * V, step = grp.threads * V;
+  int turn = 0;
+  Raw<V, uint16_t> xw[NV];
+  Raw<V, RES> rw[NV];
+  auto fetch = [&](int64_t t, int i, int n) {
+    if (i < d) {
+      xw[n].load(x + t * ldx + i);
+      if (residual) rw[n].load(residual + t * ldr + i);
+    } else {
+      xw[n].zero();
+      rw[n].zero();
+    }
+  };
+  auto sum_of = [&](int n, float (&sv)[V]) {
+    xw[n].get(sv);
+    if (residual) {
       float r[V];
-      load_row<V>(rr + i, r);
+      rw[n].get(r);
 #pragma unroll
       for (int j = 0; j < V; ++j) sv[j] += r[j];
     }
-    load_row<V>(gain + i, gv);
   };
-  auto gather = [&](const float (&sv)[V], const float (&gv)[V]) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      sum = fmaf(sv[j], sv[j], sum);
-      top = max(top, abs_bits(sv[j] * gv[j]));
-    }
+  auto gains = [&](int i, float (&gv)[V]) {   // from L1: the same for every row
+    Raw<V, uint16_t> w;
+    if (i < d) w.load_again(gain + i); else w.zero();
+    w.get(gv);
   };
-  if constexpr (LOOP) {
-    for (int i = i0; i < d; i += step) {
-      load(i, s[0], g[0]);
-      gather(s[0], g[0]);
-    }
-  } else {
+  if (!LOOP && grp.row < T) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int i = i0 + n * step;
-      if (i < d) {
-        load(i, s[n], g[n]);
+    for (int n = 0; n < NV; ++n) fetch(grp.row, i0 + n * step, n);
+  }
+  for (int64_t t = grp.row; t < T; t += grp.stride) {   // whole groups
+    float s[NV][V];
+    float sum = 0.f;
+    uint32_t top = 0;
+    // f(s, gain) over the thread's elements
+    auto each = [&](auto&& f) {
+      if constexpr (LOOP) {
+        for (int i = i0; i < d; i += step) {
+          float gv[V];
+          fetch(t, i, 0);
+          sum_of(0, s[0]);
+          gains(i, gv);
+#pragma unroll
+          for (int j = 0; j < V; ++j) f(s[0][j], gv[j]);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[n][j] = g[n][j] = 0.f;
+        for (int n = 0; n < NV; ++n) {
+          float gv[V];
+          gains(i0 + n * step, gv);
+#pragma unroll
+          for (int j = 0; j < V; ++j) f(s[n][j], gv[j]);
+        }
+      }
+    };
+    if constexpr (!LOOP) {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) sum_of(n, s[n]);
+      if (t + grp.stride < T) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) fetch(t + grp.stride, i0 + n * step, n);
       }
     }
+    each([&](float sv, float gv) {
+      sum = fmaf(sv, sv, sum);
+      top = max(top, abs_bits(sv * gv));
+    });
+    row_reduce<ONE_WARP, true>(sum, top, turn);
+    float r;
+    if (sum > kFloatMax) {
+      // the squares left the float32 range: the same on s / 2^70 (both
+      // branches are taken by whole rows)
+      sum = 0.f;
+      uint32_t unused = 0;
+      each([&](float sv, float) {
+        sv *= 0x1p-70f;
+        sum = fmaf(sv, sv, sum);
+      });
+      row_reduce<ONE_WARP, true>(sum, unused, turn);
+      r = __fdiv_rn(0x1p-70f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps * 0x1p-140f)));
+    } else {
+      r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps)));
+    }
+    if (scales && (top >= 0x7F800000u || top < 0x0D800000u)) {
+      // some |s g| is no finite number, or all are below 2^-100 and lose bits:
+      // the maximum of the values themselves
+      top = 0;
+      each([&](float sv, float gv) { top = max(top, abs_bits(sv * r * gv)); });
+      row_reduce<ONE_WARP, false>(sum, top, turn);
+    } else {
+      top = __float_as_uint(r * __uint_as_float(top));   // max|v| up to the rounding of one product
+    }
+    const float2 sc = row_scale(__uint_as_float(top));
+    if (scales && i0 == 0) scales[t] = sc.x;
+
+    auto write = [&](int i, float (&sv)[V]) {
+      float gv[V];
+      gains(i, gv);
+      if (residual_out) store_row<V>(residual_out + t * d + i, sv);
 #pragma unroll
-    for (int n = 0; n < NV; ++n) gather(s[n], g[n]);
-  }
-  row_reduce<ONE_WARP, true>(sum, top);
-  // f(s, gain) over the thread's elements once more: the two rare cases below
-  auto again = [&](auto&& f) {
+      for (int j = 0; j < V; ++j) sv[j] = sv[j] * r * gv[j];
+      if (y) store_row<V>(y + t * d + i, sv);
+      if (q) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sv[j] *= sc.y;
+        store_row<V>(q + t * d + i, sv);
+      }
+    };
     if constexpr (LOOP) {
       for (int i = i0; i < d; i += step) {
-        load(i, s[0], g[0]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f(s[0][j], g[0][j]);
+        fetch(t, i, 0);
+        sum_of(0, s[0]);
+        write(i, s[0]);
       }
     } else {
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int j = 0; j < V; ++j) f(s[n][j], g[n][j]);
+        if (i0 + n * step < d) write(i0 + n * step, s[n]);
     }
-    if (!ONE_WARP) __syncthreads();   // row_reduce's shared memory is read by now
-  };
-  float r;
-  if (sum > kFloatMax) {
-    // the squares left the float32 range: the same on s / 2^70 (both
-    // branches are taken by whole rows)
-    sum = 0.f;
-    uint32_t unused = 0;
-    again([&](float sv, float) {
-      sv *= 0x1p-70f;
-      sum = fmaf(sv, sv, sum);
-    });
-    row_reduce<ONE_WARP, true>(sum, unused);
-    r = __fdiv_rn(0x1p-70f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps * 0x1p-140f)));
-  } else {
-    r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps)));
-  }
-  if (scales && (top >= 0x7F800000u || top < 0x0D800000u)) {
-    // some |s g| is no finite number, or all are below 2^-100 and lose bits:
-    // the maximum of the values themselves
-    top = 0;
-    again([&](float sv, float gv) { top = max(top, abs_bits(sv * r * gv)); });
-    row_reduce<ONE_WARP, false>(sum, top);
-  } else {
-    top = __float_as_uint(r * __uint_as_float(top));   // max|v| up to the rounding of one product
-  }
-  const float2 sc = row_scale(__uint_as_float(top));
-  if (scales && i0 == 0) scales[t] = sc.x;
-
-  auto write = [&](int i, float (&sv)[V], const float (&gv)[V]) {
-    if (residual_out) store_row<V>(residual_out + t * d + i, sv);
-#pragma unroll
-    for (int j = 0; j < V; ++j) sv[j] = sv[j] * r * gv[j];
-    if (y) store_row<V>(y + t * d + i, sv);
-    if (q) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) sv[j] *= sc.y;
-      store_row<V>(q + t * d + i, sv);
-    }
-  };
-  if constexpr (LOOP) {
-    for (int i = i0; i < d; i += step) {
-      load(i, s[0], g[0]);
-      write(i, s[0], g[0]);
-    }
-  } else {
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (i0 + n * step < d) write(i0 + n * step, s[n], g[n]);
   }
 }
 
 template <int V, int NV, bool ONE_WARP, bool LOOP>
-__global__ void __launch_bounds__(1024) swiglu_e4m3_kernel(const uint16_t* __restrict__ gate, int64_t ldg,
-                                                           const uint16_t* __restrict__ up, int64_t ldu,
-                                                           int64_t rows, int width, uint8_t* __restrict__ q,
-                                                           float* __restrict__ scales) {
+__global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) swiglu_e4m3_kernel(
+    const uint16_t* __restrict__ gate, int64_t ldg, const uint16_t* __restrict__ up, int64_t ldu, int64_t rows,
+    int width, uint8_t* __restrict__ q, float* __restrict__ scales) {
   chain_begin();
-  int64_t t;
-  int lanes;
-  const int i0 = row_place<ONE_WARP>(&t, &lanes) * V, step = lanes * V;
-  if (ONE_WARP && t >= rows) return;
-  const uint16_t *gr = gate + t * ldg, *ur = up + t * ldu;
-  float v[NV][V], unused = 0.f;
-  uint32_t top = 0;
-  auto load = [&](int i, float (&o)[V]) {
-    float g[V], u[V];
-    load_row<V>(gr + i, g);
-    load_row<V>(ur + i, u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = g[j] * sigmoid_f32(g[j]) * u[j];
+  const Group<ONE_WARP> grp;
+  const int i0 = grp.place * V, step = grp.threads * V;
+  int turn = 0;
+  Raw<V, uint16_t> gw[NV], uw[NV];
+  auto fetch = [&](int64_t t, int i, int n) {
+    if (i < width) {
+      gw[n].load(gate + t * ldg + i);
+      uw[n].load(up + t * ldu + i);
+    } else {
+      gw[n].zero();
+      uw[n].zero();
+    }
   };
-  if constexpr (LOOP) {
-    for (int i = i0; i < width; i += step) {
-      load(i, v[0]);
+  auto value = [&](int n, float (&o)[V]) {
+    float u[V];
+    gw[n].get(o);
+    uw[n].get(u);
 #pragma unroll
-      for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[0][j]));
-    }
-  } else {
+    for (int j = 0; j < V; ++j) o[j] = o[j] * sigmoid_f32(o[j]) * u[j];
+  };
+  if (!LOOP && grp.row < rows) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      if (i0 + n * step < width) {
-        load(i0 + n * step, v[n]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[n][j] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[n][j]));
+    for (int n = 0; n < NV; ++n) fetch(grp.row, i0 + n * step, n);
   }
-  row_reduce<ONE_WARP, false>(unused, top);
-  const float2 sc = row_scale(__uint_as_float(top));
-  if (i0 == 0) scales[t] = sc.x;
-  auto write = [&](int i, float (&o)[V]) {
+  for (int64_t t = grp.row; t < rows; t += grp.stride) {   // whole groups
+    float v[NV][V], unused = 0.f;
+    uint32_t top = 0;
+    if constexpr (LOOP) {
+      for (int i = i0; i < width; i += step) {
+        fetch(t, i, 0);
+        value(0, v[0]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] *= sc.y;
-    store_row<V>(q + t * width + i, o);
-  };
-  if constexpr (LOOP) {
-    for (int i = i0; i < width; i += step) {
-      load(i, v[0]);
-      write(i, v[0]);
+        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[0][j]));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n) value(n, v[n]);
+      if (t + grp.stride < rows) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) fetch(t + grp.stride, i0 + n * step, n);
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[n][j]));
     }
-  } else {
+    row_reduce<ONE_WARP, false>(unused, top, turn);
+    const float2 sc = row_scale(__uint_as_float(top));
+    if (i0 == 0) scales[t] = sc.x;
+    auto write = [&](int i, float (&o)[V]) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (i0 + n * step < width) write(i0 + n * step, v[n]);
+      for (int j = 0; j < V; ++j) o[j] *= sc.y;
+      store_row<V>(q + t * width + i, o);
+    };
+    if constexpr (LOOP) {
+      for (int i = i0; i < width; i += step) {
+        fetch(t, i, 0);
+        value(0, v[0]);
+        write(i, v[0]);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        if (i0 + n * step < width) write(i0 + n * step, v[n]);
+    }
   }
 }
 
@@ -333,28 +379,55 @@ static bool starts_on(const void* p, int64_t ld, int64_t size, int64_t bytes) {
   return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * size % bytes == 0);
 }
 
-// Calls f(V, NV, one_warp, loop as integral constants, grid, threads) for
-// rows of `width` elements.
+// Registers a thread of `kernel` uses (a property of the code: looked up once).
+template <typename K>
+static int registers_of(K* kernel) {
+  cudaFuncAttributes attr;
+  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kernel)) != cudaSuccess) return 64;
+  return attr.numRegs > 0 ? attr.numRegs : 64;
+}
+
+// CTAs for `groups` groups: as many as are resident at once, so that a group
+// goes on to its next row with the loads in flight.
+static unsigned row_ctas(int64_t groups, int threads, int registers) {
+  const int by_regs = 65536 / (((registers + 7) & ~7) * threads), by_threads = 2048 / threads;
+  int per_sm = by_regs < by_threads ? by_regs : by_threads;
+  per_sm = per_sm < 1 ? 1 : per_sm > 32 ? 32 : per_sm;
+  const int64_t resident = int64_t(sm_count()) * per_sm;
+  return unsigned(groups < resident ? groups : resident);
+}
+
+// Calls f with the variant for rows of `width` elements (V, NV, one warp,
+// loop as integral constants), the groups and the threads of a CTA.
 template <typename F>
 static cudaError_t per_row_shape(bool wide, int64_t rows, int width, F&& f) {
   using std::integral_constant;
-  if (rows > 0x7FFFFFFF) return cudaErrorInvalidValue;
   const int v = wide ? 8 : 1;
   const int vecs = (width + v - 1) / v;
-  auto warps = [](int n) { return (n + 31) / 32 * 32; };
-  const dim3 four(unsigned((rows + 3) / 4)), one((unsigned(rows)));
-#define VX_ROWS(V, NV, W, L, grid, threads)                                                              \
-  f(integral_constant<int, V>(), integral_constant<int, NV>(), integral_constant<bool, W>(),             \
-    integral_constant<bool, L>(), grid, threads)
+  auto run = [&](auto V, auto NV, auto W, auto L) {
+    const int threads = W ? 128 : L ? 1024 : ((vecs + NV - 1) / NV + 31) / 32 * 32;
+    return f(V, NV, W, L, W ? (rows + 3) / 4 : rows, threads);
+  };
+#define VX_ROWS(V, NV, W, L)                                                                 \
+  run(integral_constant<int, V>(), integral_constant<int, NV>(), integral_constant<bool, W>(), \
+      integral_constant<bool, L>())
   if (wide) {
-    if (vecs <= 32) return VX_ROWS(8, 1, true, false, four, 128);
-    if (vecs <= 1024) return VX_ROWS(8, 1, false, false, one, warps(vecs));
-    if (vecs <= 2048) return VX_ROWS(8, 2, false, false, one, warps((vecs + 1) / 2));
-    return VX_ROWS(8, 1, false, true, one, 1024);
+    if (vecs <= 32) return VX_ROWS(8, 1, true, false);
+    // A batch that fills the GPU gives each row fewer threads with more loads
+    // each, one warp where the registers allow (no CTA barrier): norm 65,536 x
+    // 512 52 against 60 us, swiglu 20,480 x 1,024 18.8 against 21.6 us; a
+    // smaller batch spreads its rows: norm 64 x 2,048 2.1 us either way.
+    const bool many = rows >= 4 * int64_t(sm_count());
+    if (many && vecs <= 64) return VX_ROWS(8, 2, true, false);
+    if (many && vecs <= 96) return VX_ROWS(8, 3, true, false);
+    if (many && vecs <= 128) return VX_ROWS(8, 4, true, false);
+    if (vecs <= 1024 && !many) return VX_ROWS(8, 1, false, false);
+    if (vecs <= 2048) return VX_ROWS(8, 2, false, false);
+    return VX_ROWS(8, 1, false, true);
   }
-  if (vecs <= 128) return VX_ROWS(1, 4, true, false, four, 128);
-  if (vecs <= 4096) return VX_ROWS(1, 4, false, false, one, warps((vecs + 3) / 4));
-  return VX_ROWS(1, 1, false, true, one, 1024);
+  if (vecs <= 128) return VX_ROWS(1, 4, true, false);
+  if (vecs <= 4096) return VX_ROWS(1, 4, false, false);
+  return VX_ROWS(1, 1, false, true);
 #undef VX_ROWS
 }
 
@@ -365,11 +438,11 @@ static cudaError_t add_rmsnorm_as(const uint16_t* x, int64_t ldx, const RES* res
   const bool wide = d % 8 == 0 && starts_on(x, ldx, 2, 16) && starts_on(residual, ldr, sizeof(RES), 16) &&
                     starts_on(gain, 0, 2, 16) && starts_on(residual_out, d, sizeof(RES), 16) &&
                     starts_on(y, d, 2, 16) && starts_on(q, d, 1, 8);
-  return per_row_shape(wide, T, d, [&](auto v, auto nv, auto w, auto l, dim3 grid, int threads) {
-    return launch_chained(add_rmsnorm_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value, RES,
-                                             decltype(l)::value>,
-                          grid, dim3(threads), 0, st, x, ldx, residual, ldr, gain, T, d, eps, residual_out, y, q,
-                          scales);
+  return per_row_shape(wide, T, d, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
+    auto k = add_rmsnorm_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value, RES, decltype(l)::value>;
+    static const int registers = registers_of(k);
+    return launch_chained(k, dim3(row_ctas(groups, threads, registers)), dim3(threads), 0, st, x, ldx, residual, ldr,
+                          gain, T, d, eps, residual_out, y, q, scales);
   });
 }
 
@@ -389,10 +462,11 @@ cudaError_t launch_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t
   if (rows == 0) return cudaSuccess;
   const bool wide = width % 8 == 0 && starts_on(gate, ldg, 2, 16) && starts_on(up, ldu, 2, 16) &&
                     starts_on(q, width, 1, 8);
-  return per_row_shape(wide, rows, width, [&](auto v, auto nv, auto w, auto l, dim3 grid, int threads) {
-    return launch_chained(swiglu_e4m3_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value,
-                                             decltype(l)::value>,
-                          grid, dim3(threads), 0, st, gate, ldg, up, ldu, rows, width, q, scales);
+  return per_row_shape(wide, rows, width, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
+    auto k = swiglu_e4m3_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value, decltype(l)::value>;
+    static const int registers = registers_of(k);
+    return launch_chained(k, dim3(row_ctas(groups, threads, registers)), dim3(threads), 0, st, gate, ldg, up, ldu, rows,
+                          width, q, scales);
   });
 }
 

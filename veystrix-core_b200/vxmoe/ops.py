@@ -813,13 +813,22 @@ def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
 
 def _call(dev: torch.device, what: str, fn, *args) -> None:
     """fn(*args, stream) on dev's current stream, with dev current."""
-    if torch.cuda.current_device() == dev.index:
-        status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, what)
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A new contiguous tensor of t's shape (empty_like is the cheapest call
+    that allocates, and keeps strides only where they are not contiguous)."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 class AddNorm(NamedTuple):
@@ -844,10 +853,10 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
     x2, ldx = _row_view(x, "x", torch.bfloat16)
     T, d = x2.shape
     dev = x2.device
-    _same_device(dev, residual=residual, gain=gain)
-    if _bf16(gain, "gain").numel() != d:
+    gain = _bf16(gain, "gain")
+    if gain.numel() != d:
         raise ValueError("gain must have the hidden size")
-    gain = gain.contiguous()
+    _same_device(dev, residual=residual, gain=gain)
     shape = x.shape
     res_out = r2 = None
     ldr, res_type = 0, _lib.VX_DTYPE_BF16
@@ -859,12 +868,12 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
         if residual.shape != shape:
             raise ValueError(f"residual shape {tuple(residual.shape)} != {tuple(shape)}")
         r2, ldr = _row_view(residual, "residual", residual.dtype)
-        res_out = torch.empty(shape, dtype=residual.dtype, device=dev)
-    y = torch.empty(shape, dtype=torch.bfloat16, device=dev) if output != "e4m3" else None
+        res_out = _like(x, residual.dtype)
+    y = _like(x, torch.bfloat16) if output != "e4m3" else None
     q = scales = None
     if output != "bf16":
-        q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
-        scales = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+        q = _like(x, torch.float8_e4m3fn)
+        scales = x2.new_empty(shape[:-1], dtype=torch.float32)
     _call(dev, "add_rms_norm", _lib.load().vx_add_rmsnorm, x2.data_ptr(), ldx, _ptr(r2), res_type, ldr,
           gain.data_ptr(), T, d, float(eps), _ptr(res_out), _ptr(y), _ptr(q), _ptr(scales))
     return AddNorm(y, res_out, q, scales)
@@ -887,8 +896,8 @@ def swiglu_e4m3(gate: torch.Tensor, up: torch.Tensor) -> E4M3Rows:
     dev = g2.device
     _same_device(dev, up=u2)
     rows, width = g2.shape
-    q = torch.empty(gate.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scales = torch.empty(gate.shape[:-1], dtype=torch.float32, device=dev)
+    q = _like(gate, torch.float8_e4m3fn)
+    scales = g2.new_empty(gate.shape[:-1], dtype=torch.float32)
     _call(dev, "swiglu_e4m3", _lib.load().vx_swiglu_e4m3, g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width,
           q.data_ptr(), scales.data_ptr())
     return E4M3Rows(q, scales)
@@ -942,7 +951,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     if slots < 1:
         raise ValueError("slots must be at least 1")
     if out is None:
-        out = torch.empty((P, N), dtype=torch.bfloat16, device=dev)
+        out = x.new_empty((P, N), dtype=torch.bfloat16)
     else:
         _require_cuda(out, "out")
         if out.dtype != torch.bfloat16:
@@ -997,7 +1006,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     scales = _vector(scales, "scales", torch.float32, (L,))
     ranks = _vector(ranks, "ranks", torch.int32, (L,))
     if out is None:
-        out = torch.empty(y.shape, dtype=torch.bfloat16, device=dev)
+        out = _like(y, torch.bfloat16)
         ldo = N
     else:
         o2, ldo = _row_view(out, "out", torch.bfloat16)
