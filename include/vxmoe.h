@@ -387,9 +387,9 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
  * ranks may be NULL (1 and R).  A token whose adapter is outside [0, L) gets
  * y.  Sums in float32, one rounding.  out may be y itself (ldo == ldy).  K
  * and R are multiples of 8, R <= 256, L <= 4096; x, a and b start on
- * 16-byte boundaries, as do the rows of x.  The workspace is needed above
- * 256 tokens (vx_lora_add_workspace is 0 below). */
-size_t vx_lora_add_workspace(int64_t T, int32_t L);
+ * 16-byte boundaries, as do the rows of x.  The workspace (16-byte aligned)
+ * is needed above 256 tokens (vx_lora_add_workspace is 0 below). */
+size_t vx_lora_add_workspace(int64_t T, int32_t L, int32_t R);
 int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a,
                 const uint16_t* b, const int32_t* adapters, const float* scales, const int32_t* ranks,
                 int32_t L, int64_t T, int32_t K, int32_t N, int32_t R, uint16_t* out, int64_t ldo,

@@ -76,11 +76,11 @@ def test_lora_add_refusals(lib):
                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(x=ODD), dict(a=ODD), dict(b=ODD)):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw
     assert call(T=0, x=None, y=None, out=None) == _lib.VX_OK
-    need = lib.vx_lora_add_workspace(300, 2)
-    assert lib.vx_lora_add_workspace(256, 2) == 0 and need >= 2 * 300 * 4
+    need = lib.vx_lora_add_workspace(300, 2, 8)
+    assert lib.vx_lora_add_workspace(256, 2, 8) == 0 and need >= 2 * 300 * 4
     for kw in (dict(), dict(ws=P16, nbytes=need - 1), dict(ws=ODD, nbytes=need)):
         assert call(T=300, **kw) == _lib.VX_EWORKSPACE, kw
-    assert lib.vx_lora_add_workspace(-1, 2) == lib.vx_lora_add_workspace(1, 0) == 0
+    assert lib.vx_lora_add_workspace(-1, 2, 8) == lib.vx_lora_add_workspace(300, 0, 8) == 0
 
 
 def test_python_layer_takes_cuda_tensors_only():

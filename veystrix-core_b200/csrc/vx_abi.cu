@@ -1129,9 +1129,9 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 
-size_t vx_lora_add_workspace(int64_t T, int32_t L) {
-  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters) return 0;
-  return size_t(lora_workspace_bytes(T, L));
+size_t vx_lora_add_workspace(int64_t T, int32_t L, int32_t R) {
+  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || R < 1 || R > kLoraMaxRank) return 0;
+  return size_t(lora_workspace_bytes(T, L, R));
 }
 
 int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a, const uint16_t* b,
@@ -1145,8 +1145,8 @@ int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, 
   if (!y || !x || !a || !b || !adapters || !out || !aligned16(x) || !aligned16(a) || !aligned16(b))
     return VX_EINVAL_SHAPE;
   LoraArgs args{y, ldy, x, ldx, a, b, adapters, scales, ranks, L, K, N, R, T, out, ldo};
-  const size_t need = vx_lora_add_workspace(T, L);
-  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4))
+  const size_t need = vx_lora_add_workspace(T, L, R);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return VX_EWORKSPACE;
   cudaError_t e = launch_lora(args, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);

@@ -406,7 +406,7 @@ struct LoraArgs {
   uint16_t* out;                // [T][ldo]
   int64_t ldo;
 };
-int64_t lora_workspace_bytes(int64_t T, int L);   // 0 for the batches that group themselves
+int64_t lora_workspace_bytes(int64_t T, int L, int R);   // 0 for the batches that group themselves
 cudaError_t launch_lora(const LoraArgs& a, void* workspace, cudaStream_t st);
 
 cudaError_t launch_swiglu(const uint16_t* g, const uint16_t* u, uint16_t* out, int64_t n,

@@ -134,7 +134,7 @@ SIGNATURES = {
                                          c_int32, c_int64, P, c_int64, P]),
     "vx_lora_add": (ctypes.c_int, [P, c_int64, P, c_int64, P, P, P, P, P, c_int32, c_int64, c_int32, c_int32,
                                    c_int32, P, c_int64, P, c_size_t, P]),
-    "vx_lora_add_workspace": (c_size_t, [c_int64, c_int32]),
+    "vx_lora_add_workspace": (c_size_t, [c_int64, c_int32, c_int32]),
     "vx_profile_enable": (ctypes.c_int, [ctypes.c_int]),
     "vx_profile_read": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_int,
                                        ctypes.POINTER(ctypes.c_double),

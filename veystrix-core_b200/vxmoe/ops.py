@@ -1013,7 +1013,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         if out.shape != y.shape or o2.data_ptr() != out.data_ptr():
             raise ValueError(f"out must be rows of shape {tuple(y.shape)}, got {tuple(out.shape)}")
     lib = _lib.load()
-    nbytes = lib.vx_lora_add_workspace(T, L)
+    nbytes = lib.vx_lora_add_workspace(T, L, R)
     # its own allocation: a captured graph keeps it in its own pool
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call(dev, "lora_add", lib.vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
