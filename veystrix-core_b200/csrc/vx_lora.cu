@@ -18,13 +18,15 @@
 //
 // Up to kLoraSmall tokens: one launch.  The batch is grouped inside the
 // kernel; a cluster of C CTAs shares an item of 16 tokens: CTA i forms A_e x
-// over its part of K, the cluster adds the parts (distributed shared memory,
-// in CTA order), and CTA i writes its part of N.  B and y are on their way
-// (L2 prefetches, then registers) while h is being summed.
+// over its part of K and stores it into the shared memory of every CTA
+// (st.async on the receiver's mbarrier: a cluster barrier costs 1,400 cycles,
+// and two would stand here), each adds the parts in CTA order, and CTA i
+// writes its part of N.  B and y are on their way while h is being summed.
 //
 // Above: lora_group_kernel sorts the batch into items of 32 tokens,
 // lora_shrink_kernel (a CTA an item) writes h as bf16 pairs, and
-// lora_expand_kernel (a CTA an item and kExpandCols outputs) streams y.
+// lora_expand_kernel (a CTA an item and 512 or 1,024 outputs) streams y.
+#include "vx_async.cuh"
 #include "vx_common.cuh"
 #include "vx_launch.h"
 
@@ -32,7 +34,6 @@ namespace vx {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraRankChunk = 64;     // components whose sums a warp holds in registers
 constexpr int kLoraSmall = kLoraThreads;
 
 VX_DEVICE uint32_t lora_cluster_rank() {
@@ -45,16 +46,31 @@ VX_DEVICE uint32_t lora_cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-VX_DEVICE void lora_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+VX_DEVICE void lora_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+VX_DEVICE void lora_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Four floats to the same place in CTA `rank`, counted on its barrier `bar`.
+VX_DEVICE void push4(const float* p, uint64_t* bar, uint32_t rank, float4 v) {
+  uint32_t to, on;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(on) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(on)
+               : "memory");
 }
-VX_DEVICE float peer_f32(const float* p, uint32_t rank) {   // the same place in CTA `rank`
-  const uint32_t own = static_cast<uint32_t>(__cvta_generic_to_shared(p));
-  uint32_t addr;
-  float v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(own), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Bounded wait for phase 0 of `bar` (false after a second).
+VX_DEVICE bool lora_wait(uint64_t* bar) {
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0; selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(smem_u32(bar))
+        : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255 && global_ns() - t0 > kWaitLimitNs) return false;
+  }
+  return false;
 }
 
 VX_DEVICE int lora_id(const LoraArgs& a, int64_t t) {
@@ -100,21 +116,21 @@ VX_DEVICE void store8(uint16_t* row, int n, int N, const float (&v)[8]) {
   }
 }
 
-__host__ __device__ constexpr int lora_part_floats(int tm, int R) {   // the warps' sums of a rank chunk
-  return kLoraWarps * tm * (R < kLoraRankChunk ? R : kLoraRankChunk);
-}
-__host__ __device__ constexpr int lora_frag_bytes(int mt, int R) { return (R + 15) / 16 * mt * 1024; }
+__host__ __device__ constexpr int lora_frag_bytes(int mt, int R) { return (R + 31) / 32 * mt * 2048; }
 
 // Components of adapter e that count.
 VX_DEVICE int lora_rank(const LoraArgs& a, int e) {
   return e < 0 ? 0 : a.ranks ? min(max(__ldg(a.ranks + e), 0), a.R) : a.R;
 }
 
-// sums[row][r] (TM x R floats) = A_e x over the 32-input blocks first, first
-// + stride, ... of the CTA's warps; part: lora_part_floats.
-template <int MT>
-VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, int first, int stride, float* part,
-                           float* sums) {
+// A_e x of the item's n tokens over the 32-input blocks first, first + stride,
+// ... of the CTA's warps, 8 * NT components at a time; out(row, r, v) gets
+// four neighbouring sums of the CTA.  part: lora_part_floats.  AHEAD: the
+// next block's operands are loaded before the present one's MMAs.  ready() is
+// called by every thread once, before the first out().
+template <int MT, int NT, bool AHEAD, typename G, typename F>
+VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, int n, int first, int stride,
+                           float* part, G&& ready, F&& out) {
   constexpr int TM = 16 * MT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint16_t* xrow[2 * MT];
@@ -125,22 +141,23 @@ VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, i
   }
   const uint16_t* A = a.a + int64_t(e) * a.R * a.K;
   const int blocks = (a.K + 31) / 32;
-  for (int r0 = 0; r0 < rank; r0 += kLoraRankChunk) {
-    const int cols = min(kLoraRankChunk, rank - r0), tiles = (cols + 7) / 8;
-    float acc[MT][8][4] = {};
-    for (int kb = first; kb < blocks; kb += stride) {
+  for (int r0 = 0; r0 < rank; r0 += 8 * NT) {
+    const int tiles = (min(8 * NT, rank - r0) + 7) / 8;
+    float acc[MT][NT][4] = {};
+    auto load = [&](int kb, uint4 (&xf)[2 * MT], uint4 (&af)[NT]) {
       const int k = kb * 32 + c * 8;
-      uint4 xf[2 * MT], af[8];
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i)
         xf[i] = xrow[i] && k < a.K ? ldg_nc(xrow[i] + k) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < NT; ++j) {
         const int r = r0 + 8 * j + g;
-        af[j] = j < tiles && r < rank && k < a.K ? ldg_nc(A + int64_t(r) * a.K + k) : make_uint4(0, 0, 0, 0);
+        af[j] = r < rank && k < a.K ? ldg_nc(A + int64_t(r) * a.K + k) : make_uint4(0, 0, 0, 0);
       }
+    };
+    auto multiply = [&](const uint4 (&xf)[2 * MT], const uint4 (&af)[NT]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < NT; ++j) {
         if (j >= tiles) break;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
@@ -148,26 +165,51 @@ VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, i
           mma16816(acc[m][j], xf[2 * m].z, xf[2 * m + 1].z, xf[2 * m].w, xf[2 * m + 1].w, af[j].z, af[j].w);
         }
       }
+    };
+    uint4 xf[2 * MT], af[NT];
+    if constexpr (AHEAD) {
+      uint4 xn[2 * MT], an[NT];
+      int kb = first;
+      if (kb < blocks) load(kb, xf, af);
+      while (kb < blocks) {   // two blocks a turn, so that neither set is copied
+        if (kb + stride < blocks) load(kb + stride, xn, an);
+        multiply(xf, af);
+        kb += stride;
+        if (kb >= blocks) break;
+        if (kb + stride < blocks) load(kb + stride, xf, af);
+        multiply(xn, an);
+        kb += stride;
+      }
+    } else {
+      for (int kb = first; kb < blocks; kb += stride) {
+        load(kb, xf, af);
+        multiply(xf, af);
+      }
     }
-    const int pitch = min(kLoraRankChunk, a.R);
-    float* mine = part + warp * TM * pitch;
+    constexpr int kPitch = 8 * NT;
+    float* mine = part + warp * TM * kPitch;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < NT; ++j) {
       if (j >= tiles) break;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        float* p = mine + (16 * m + g) * pitch + 8 * j + 2 * c;
+        float* p = mine + (16 * m + g) * kPitch + 8 * j + 2 * c;
         *reinterpret_cast<float2*>(p) = make_float2(acc[m][j][0], acc[m][j][1]);
-        *reinterpret_cast<float2*>(p + 8 * pitch) = make_float2(acc[m][j][2], acc[m][j][3]);
+        *reinterpret_cast<float2*>(p + 8 * kPitch) = make_float2(acc[m][j][2], acc[m][j][3]);
       }
     }
     __syncthreads();
-    for (int i = tid; i < TM * tiles * 8; i += kLoraThreads) {
-      const int row = i / (tiles * 8), col = i - row * (tiles * 8);
-      float s = 0.f;
+    if (r0 == 0) ready();
+    for (int i = tid; i < n * 2 * NT; i += kLoraThreads) {
+      const int row = i / (2 * NT), col = i % (2 * NT) * 4;
+      if (col >= tiles * 8) continue;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kLoraWarps; ++w) s += part[(w * TM + row) * pitch + col];
-      sums[row * a.R + r0 + col] = s;
+      for (int w = 0; w < kLoraWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (w * TM + row) * kPitch + col);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+      }
+      out(row, r0 + col, s);
     }
     __syncthreads();
   }
@@ -179,35 +221,29 @@ VX_DEVICE void lora_split(float v, uint16_t* hi, uint16_t* lo) {
   *lo = (*hi & 0x7F80u) != 0x7F80u ? f32_to_bf16(v - bf16_to_f32(*hi)) : uint16_t(0);
 }
 // Place of h's component r of item row `row` in the fragments [16 components]
-// [MT][hi, lo][lane][8 halves]: component q of 16 belongs to the lanes q/4 of
-// four, like their reads of B; the lo half lies 256 halves on.
+// [MT][hi, lo][lane][8 halves].  Of every 32 components the lanes c of four
+// own 8 c .. 8 c + 7, as one 16-byte read of B brings them: the first four in
+// the first MMA's 16, the others in the second's.  lo lies 256 halves on.
 template <int MT>
 VX_DEVICE int lora_frag_at(int row, int r) {
-  const int q = r & 15, reg = (q & 2) + ((row & 15) >> 3), lane = (row & 7) * 4 + (q >> 2);
-  return (((r >> 4) * MT + (row >> 4)) * 64 + lane) * 8 + reg * 2 + (q & 1);
+  const int kb = (r >> 5) * 2 + ((r >> 2) & 1), lane = (row & 7) * 4 + ((r >> 3) & 3);
+  const int reg = (r & 2) + ((row & 15) >> 3);
+  return ((kb * MT + (row >> 4)) * 64 + lane) * 8 + reg * 2 + (r & 1);
 }
 
-// B of one 32-output block: kExpandKb blocks of 16 components x 4 MMA tiles.
+// B of one 32-output block: KB pairs of 16 components x 4 MMA tiles.
 // Column q of MMA tile j is output 8 (q/2) + 2 j + q%2 of the 32, so a lane
-// ends up with 8 neighbours.  Components from `rank` on count as zero.
-constexpr int kExpandKb = 2;
-VX_DEVICE void load_b(const LoraArgs& a, const uint16_t* B, int rank, int nb, int kb0, uint2 (&bf)[kExpandKb][4]) {
+// ends up with 8 neighbours.
+template <int KB>
+VX_DEVICE void load_b(const LoraArgs& a, const uint16_t* B, int rank, int nb, int kb0, uint4 (&bf)[KB][4]) {
   const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
 #pragma unroll
-  for (int u = 0; u < kExpandKb; ++u) {
+  for (int u = 0; u < KB; ++u) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = nb * 32 + 8 * (g >> 1) + 2 * j + (g & 1), r = (kb0 + u) * 16 + 4 * c;
-      uint2 v = make_uint2(0, 0);
-      if (r < rank && row < a.N) {
-        v = __ldg(reinterpret_cast<const uint2*>(B + int64_t(row) * a.R + r));
-        const int left = rank - r;
-        if (left < 4) {
-          if (left < 2) v.x &= 0xFFFFu;
-          v.y = left < 3 ? 0u : v.y & 0xFFFFu;
-        }
-      }
-      bf[u][j] = v;
+      const int row = nb * 32 + 8 * (g >> 1) + 2 * j + (g & 1), r = (kb0 + u) * 32 + 8 * c;
+      bf[u][j] = r < rank && row < a.N ? __ldg(reinterpret_cast<const uint4*>(B + int64_t(row) * a.R + r))
+                                       : make_uint4(0, 0, 0, 0);
     }
   }
 }
@@ -219,24 +255,36 @@ VX_DEVICE void load_y(const LoraArgs& a, const int (&t)[2 * MT], int nb, Eight<W
     if (t[i] >= 0 && (!WIDE || n < a.N)) y[i].load(a.y + t[i] * a.ldy, n, a.N);
 }
 // out = y + B h for one block whose y and first B are loaded.
-template <int MT, bool WIDE>
+template <int MT, int KB, bool WIDE>
 VX_DEVICE void lora_expand(const LoraArgs& a, const uint16_t* B, int rank, const uint4* frag, const int (&t)[2 * MT],
-                           int nb, const Eight<WIDE> (&y)[2 * MT], uint2 (&bf)[kExpandKb][4]) {
-  const int lane = threadIdx.x & 31, n = nb * 32 + 8 * (lane & 3), kbs = (rank + 15) / 16;
+                           int nb, const Eight<WIDE> (&y)[2 * MT], uint4 (&bf)[KB][4]) {
+  const int lane = threadIdx.x & 31, c = lane & 3, n = nb * 32 + 8 * c, kbs = (rank + 31) / 32;
   float acc[MT][4][4] = {};
-  for (int kb0 = 0; kb0 < kbs; kb0 += kExpandKb) {
-    if (kb0 > 0) load_b(a, B, rank, nb, kb0, bf);
+  for (int kb0 = 0; kb0 < kbs; kb0 += KB) {
+    if (kb0 > 0) load_b<KB>(a, B, rank, nb, kb0, bf);
 #pragma unroll
-    for (int u = 0; u < kExpandKb; ++u) {
+    for (int u = 0; u < KB; ++u) {
       if (kb0 + u >= kbs) break;
+      // components behind the adapter's rank count as zero, whatever they hold
+      const int left = rank - ((kb0 + u) * 32 + 8 * c);
+      if (left < 8) {
+        auto keep = [&](int i) { return left > 2 * i + 1 ? ~0u : left > 2 * i ? 0xFFFFu : 0u; };
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4* h = frag + ((kb0 + u) * MT + m) * 64 + lane;
-        const uint4 hi = h[0], lo = h[32];
+        for (int j = 0; j < 4; ++j)
+          bf[u][j] = make_uint4(bf[u][j].x & keep(0), bf[u][j].y & keep(1), bf[u][j].z & keep(2), bf[u][j].w & keep(3));
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16816(acc[m][j], hi.x, hi.y, hi.z, hi.w, bf[u][j].x, bf[u][j].y);
-          mma16816(acc[m][j], lo.x, lo.y, lo.z, lo.w, bf[u][j].x, bf[u][j].y);
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint4* h = frag + ((2 * (kb0 + u) + half) * MT + m) * 64 + lane;
+          const uint4 hi = h[0], lo = h[32];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t b0 = half ? bf[u][j].z : bf[u][j].x, b1 = half ? bf[u][j].w : bf[u][j].y;
+            mma16816(acc[m][j], hi.x, hi.y, hi.z, hi.w, b0, b1);
+            mma16816(acc[m][j], lo.x, lo.y, lo.z, lo.w, b0, b1);
+          }
         }
       }
     }
@@ -253,10 +301,41 @@ VX_DEVICE void lora_expand(const LoraArgs& a, const uint16_t* B, int rank, const
     store8<WIDE>(a.out + t[i] * a.ldo, n, a.N, v);
   }
 }
+// The 32-output blocks first, first + stride, ... below `end`, each one's y
+// and B loaded before its predecessor is computed; the first block's are
+// loaded by the caller.
+template <int MT, int KB, bool WIDE>
+VX_DEVICE void lora_expand_all(const LoraArgs& a, const uint16_t* B, int rank, const uint4* frag,
+                               const int (&t)[2 * MT], int first, int stride, int end, Eight<WIDE> (&y)[2 * MT],
+                               uint4 (&bf)[KB][4]) {
+  Eight<WIDE> yn[2 * MT];
+  uint4 bn[KB][4];
+  int nb = first;
+  while (nb * 32 < end) {   // two blocks a turn, so that neither set is copied
+    int next = nb + stride;
+    if (next * 32 < end) {
+      load_y<MT, WIDE>(a, t, next, yn);
+      load_b<KB>(a, B, rank, next, 0, bn);
+    }
+    lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, y, bf);
+    nb = next;
+    if (nb * 32 >= end) break;
+    next = nb + stride;
+    if (next * 32 < end) {
+      load_y<MT, WIDE>(a, t, next, y);
+      load_b<KB>(a, B, rank, next, 0, bf);
+    }
+    lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, yn, bn);
+    nb = next;
+  }
+}
 
 // ---- small batches: one launch ------------------------------------------------
 
-static int lora_small_smem(int R) { return (lora_part_floats(16, R) + 16 * R) * 4 + lora_frag_bytes(1, R); }
+constexpr int kSmallNt = 8, kSmallKb = 2;
+constexpr int kSmallPart = kLoraWarps * 16 * 8 * kSmallNt;   // floats
+// the warps' sums, the parts of C CTAs [C][16][R], the fragments
+static int lora_small_smem(int R, int C) { return (kSmallPart + C * 16 * R) * 4 + lora_frag_bytes(1, R); }
 
 template <bool WIDE>
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraArgs a) {
@@ -266,6 +345,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
   __shared__ int tok[TM];          // the item's tokens, -1 behind the last
   __shared__ __align__(16) int s_ids[kLoraSmall];
   __shared__ int s_lead[kLoraWarps], s_item[2];
+  __shared__ __align__(8) uint64_t arrived;   // bytes of the cluster's parts
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = int(lora_cluster_size()), cta = int(lora_cluster_rank());
   const int item = int(blockIdx.x) / C, T = int(a.T);
@@ -275,6 +355,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
   const int mine = tid < T ? lora_id(a, tid) : -2;
   s_ids[tid] = mine;
   if (tid < TM) tok[tid] = -1;
+  if (tid == 0) {
+    mbar_init(smem_u32(&arrived));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   int before = __popc(__match_any_sync(0xFFFFFFFFu, mine) & ((1u << lane) - 1u));
   __syncthreads();
   if (tid < T) {
@@ -297,165 +381,151 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
   if (leads && number == item) s_item[0] = mine, s_item[1] = before / TM;
   __syncthreads();
   const int e = s_item[0];
-  if (tid < T && mine == e && before / TM == s_item[1]) tok[before % TM] = tid;
-  __syncthreads();
+  const bool member = tid < T && mine == e && before / TM == s_item[1];
+  if (member) tok[before % TM] = tid;
+  const int n = __syncthreads_count(member);
   const int rank = lora_rank(a, e);
+  __syncwarp();
+  if (rank > 0) lora_cluster_arrive();   // the barrier above is initialised
 
   float* part = reinterpret_cast<float*>(smem_raw);
-  float* sums = part + lora_part_floats(TM, a.R);
-  uint4* frag = reinterpret_cast<uint4*>(sums + TM * a.R);
+  float* parts = part + kSmallPart;
+  uint4* frag = reinterpret_cast<uint4*>(parts + C * TM * a.R);
   const uint16_t* B = a.b + int64_t(e < 0 ? 0 : e) * a.N * a.R;
   const int nb0 = cta * kLoraWarps + warp, stride = C * kLoraWarps;
-  // lane i: row i of the blocks of B that this warp reads later
-  for (int nb = nb0; nb * 32 < a.N; nb += stride) {
-    if (nb * 32 + lane < a.N)
-      for (int r = 0; r < rank; r += 64)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(B + int64_t(nb * 32 + lane) * a.R + r));
-  }
-  if (rank > 0) lora_shrink<1>(a, e, rank, tok, nb0, stride, part, sums);
-
   int t[2];
   Eight<WIDE> y[2];
-  uint2 bf[kExpandKb][4];
+  uint4 bf[kSmallKb][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i) t[i] = tok[8 * i + (lane >> 2)];
+  if (rank > 0) {
+    if (tid == 0) mbar_expect(smem_u32(&arrived), uint32_t(C * n * ((rank + 7) / 8) * 32));
+    // the cluster barrier is a warp's, not a thread's: whole warps wait at it
+    lora_shrink<1, kSmallNt, false>(
+        a, e, rank, tok, n, nb0, stride, part, [] { lora_cluster_wait(); },
+        [&](int row, int r, float4 v) {
+          for (int q = 0; q < C; ++q) push4(parts + (cta * TM + row) * a.R + r, &arrived, q, v);
+        });
+  }
   if (nb0 * 32 < a.N) {
     load_y<1, WIDE>(a, t, nb0, y);
-    load_b(a, B, rank, nb0, 0, bf);
+    load_b<kSmallKb>(a, B, rank, nb0, 0, bf);
   }
-  // h of the whole item
   if (rank > 0) {
-    if (C > 1) lora_cluster_sync();
-    const int cols = (rank + 15) & ~15;
-    const float scale = a.scales ? __ldg(a.scales + e) : 1.0f;
+    const bool ok = lora_wait(&arrived);
+    const int cols = (rank + 31) & ~31;
+    const float scale = ok ? a.scales ? __ldg(a.scales + e) : 1.0f : __uint_as_float(0x7FC00000u);
     uint16_t* f = reinterpret_cast<uint16_t*>(frag);
-    for (int i = tid; i < TM * cols; i += kLoraThreads) {
+    for (int i = tid; i < n * cols; i += kLoraThreads) {   // rows behind the last token are not stored
       const int row = i / cols, r = i - row * cols;
       float v = 0.f;
-      if (r < rank) {
-        if (C == 8) {   // all parts on their way before the first is added
-          float p[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) p[q] = peer_f32(sums + row * a.R + r, q);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v += p[q];
-        } else {
-          for (int q = 0; q < C; ++q) v += peer_f32(sums + row * a.R + r, q);
-        }
-      }
+      if (r < rank)
+        for (int q = 0; q < C; ++q) v += parts[(q * TM + row) * a.R + r];
       uint16_t* at = f + lora_frag_at<1>(row, r);
       lora_split(v * scale, at, at + 256);
     }
-    if (C > 1)
-      lora_cluster_sync();   // nobody leaves while its sums are read
-    else
-      __syncthreads();
+    __syncthreads();
   }
-  for (int nb = nb0; nb * 32 < a.N; nb += stride) {
-    if (nb != nb0) {
-      load_y<1, WIDE>(a, t, nb, y);
-      load_b(a, B, rank, nb, 0, bf);
-    }
-    lora_expand<1, WIDE>(a, B, rank, frag, t, nb, y, bf);
-  }
+  lora_expand_all<1, kSmallKb, WIDE>(a, B, rank, frag, t, nb0, stride, a.N, y, bf);
 }
 
 // ---- large batches ------------------------------------------------------------
 
 constexpr int kLargeMt = 2, kLargeTm = 16 * kLargeMt;
-constexpr int kExpandCols = 512;       // outputs of an expanding CTA
 
-// An item of lora_group_kernel: {adapter or -1, first place of `order`, tokens}.
-struct LoraItem {
-  int e, begin, n;
-};
-VX_DEVICE LoraItem lora_item(const int32_t* items, int i) {
-  const int32_t* p = items + 1 + 3 * i;
-  return {__ldg(p), __ldg(p + 1), __ldg(p + 2)};
-}
+constexpr int kLargeNt = 4, kLargeKb = 1;
+constexpr int kLargePart = kLoraWarps * kLargeTm * 8 * kLargeNt;   // floats
 
-static int lora_shrink_smem(int R) { return (lora_part_floats(kLargeTm, R) + kLargeTm * R) * 4; }
+// An item of lora_group_kernel: {adapter or -1, first place of `order`,
+// tokens (0: no item), rank}.
 
 // h [place of order][16 components][hi, lo][16] of every item.
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const LoraArgs a,
                                                                       const int32_t* __restrict__ order,
-                                                                      const int32_t* __restrict__ items,
+                                                                      const int4* __restrict__ items,
                                                                       uint16_t* __restrict__ h) {
   chain_begin();
-  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ __align__(16) float part[kLargePart];
   __shared__ int tok[kLargeTm];
   const int tid = threadIdx.x;
-  if (int(blockIdx.x) >= __ldg(items)) return;
-  const LoraItem it = lora_item(items, blockIdx.x);
-  const int rank = lora_rank(a, it.e);
-  if (rank == 0) return;
-  if (tid < kLargeTm) tok[tid] = tid < it.n ? __ldg(order + it.begin + tid) : -1;
+  const int4 it = __ldg(items + blockIdx.x);
+  const int e = it.x, begin = it.y, n = it.z, rank = it.w;
+  if (n == 0 || rank == 0) return;
+  if (tid < kLargeTm) tok[tid] = tid < n ? __ldg(order + begin + tid) : -1;
+  const float scale = a.scales ? __ldg(a.scales + e) : 1.0f;
   __syncthreads();
-  float* part = reinterpret_cast<float*>(smem_raw);
-  float* sums = part + lora_part_floats(kLargeTm, a.R);
-  lora_shrink<kLargeMt>(a, it.e, rank, tok, tid >> 5, kLoraWarps, part, sums);
-  const int cols = (rank + 15) & ~15, pitch = ((a.R + 15) & ~15) * 2;
-  const float scale = a.scales ? __ldg(a.scales + it.e) : 1.0f;
-  for (int i = tid; i < it.n * cols; i += kLoraThreads) {
-    const int row = i / cols, r = i - row * cols;
-    uint16_t* p = h + int64_t(it.begin + row) * pitch + (r >> 4) * 32 + (r & 15);
-    lora_split(r < rank ? sums[row * a.R + r] * scale : 0.f, p, p + 16);
-  }
+  const int pitch = ((a.R + 15) & ~15) * 2;
+  lora_shrink<kLargeMt, kLargeNt, true>(
+      a, e, rank, tok, n, tid >> 5, kLoraWarps, part, [] {},
+      [&](int row, int r, float4 v) {
+        const float f[4] = {v.x, v.y, v.z, v.w};
+        uint16_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lora_split(r + i < rank ? f[i] * scale : 0.f, &hi[i], &lo[i]);
+        uint16_t* p = h + int64_t(begin + row) * pitch + (r >> 4) * 32 + (r & 15);
+        *reinterpret_cast<uint2*>(p) = make_uint2(hi[0] | uint32_t(hi[1]) << 16, hi[2] | uint32_t(hi[3]) << 16);
+        *reinterpret_cast<uint2*>(p + 16) = make_uint2(lo[0] | uint32_t(lo[1]) << 16, lo[2] | uint32_t(lo[3]) << 16);
+      });
 }
 
 template <bool WIDE>
-__global__ void __launch_bounds__(kLoraThreads, 3) lora_expand_kernel(const LoraArgs a,
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const LoraArgs a,
                                                                       const int32_t* __restrict__ order,
-                                                                      const int32_t* __restrict__ items,
-                                                                      const uint16_t* __restrict__ h) {
+                                                                      const int4* __restrict__ items,
+                                                                      const uint16_t* __restrict__ h, int cols) {
   chain_begin();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (int(blockIdx.x) >= __ldg(items)) return;
-  const LoraItem it = lora_item(items, blockIdx.x);
-  const int rank = lora_rank(a, it.e);
+  const int4 it = __ldg(items + blockIdx.x);
+  const int e = it.x, begin = it.y, n = it.z, rank = it.w;
+  if (n == 0) return;
   int t[2 * kLargeMt];
 #pragma unroll
   for (int i = 0; i < 2 * kLargeMt; ++i) {
     const int row = 8 * i + (lane >> 2);
-    t[i] = row < it.n ? __ldg(order + it.begin + row) : -1;
+    t[i] = row < n ? __ldg(order + begin + row) : -1;
   }
-  // the fragments: thread = 4 components of a row, hi or lo
+  const uint16_t* B = a.b + int64_t(e < 0 ? 0 : e) * a.N * a.R;
+  const int end = min(a.N, int(blockIdx.y + 1) * cols), nb0 = int(blockIdx.y) * (cols / 32) + warp;
+  Eight<WIDE> y[2 * kLargeMt];
+  uint4 bf[kLargeKb][4];
+  if (nb0 * 32 < end) {
+    load_b<kLargeKb>(a, B, rank, nb0, 0, bf);
+    load_y<kLargeMt, WIDE>(a, t, nb0, y);
+  }
+  // the fragments: a thread brings 4 components of a row, hi or lo.  What
+  // shrink did not write (above the rank's last 8) counts as zero: its column
+  // of B does, and h must be finite there.
   uint4* frag = reinterpret_cast<uint4*>(smem_raw);
-  const int kbs = (rank + 15) / 16, pitch = ((a.R + 15) & ~15) * 2;
-  for (int i = tid; i < kLargeTm * kbs * 8; i += kLoraThreads) {
-    const int row = i / (kbs * 8), piece = i - row * (kbs * 8), kb = piece >> 3, lo = (piece >> 2) & 1, q = piece & 3;
+  const int pieces = (rank + 31) / 32 * 16, pitch = ((a.R + 15) & ~15) * 2;   // 8 of hi, 8 of lo for 32 components
+  for (int i = tid; i < kLargeTm * pieces; i += kLoraThreads) {
+    const int row = i / pieces, piece = i - row * pieces, r = (piece >> 1) * 4, lo = piece & 1;
     uint2 v = make_uint2(0, 0);
-    if (row < it.n)
-      v = *reinterpret_cast<const uint2*>(h + int64_t(it.begin + row) * pitch + kb * 32 + lo * 16 + q * 4);
-    uint32_t* p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(frag) +
-                                              lora_frag_at<kLargeMt>(row, kb * 16 + q * 4) + lo * 256);
+    if (row < n && r < rank)
+      v = *reinterpret_cast<const uint2*>(h + int64_t(begin + row) * pitch + (r >> 4) * 32 + lo * 16 + (r & 15));
+    uint32_t* p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(frag) + lora_frag_at<kLargeMt>(row, r) +
+                                              lo * 256);
     p[0] = v.x;   // components 0, 1 of the four
     p[2] = v.y;   // 2, 3: two registers on
   }
   __syncthreads();
-  const uint16_t* B = a.b + int64_t(it.e < 0 ? 0 : it.e) * a.N * a.R;
-  const int end = min(a.N, int(blockIdx.y + 1) * kExpandCols);
-  for (int nb = int(blockIdx.y) * (kExpandCols / 32) + warp; nb * 32 < end; nb += kLoraWarps) {
-    Eight<WIDE> y[2 * kLargeMt];
-    uint2 bf[kExpandKb][4];
-    load_y<kLargeMt, WIDE>(a, t, nb, y);
-    load_b(a, B, rank, nb, 0, bf);
-    lora_expand<kLargeMt, WIDE>(a, B, rank, frag, t, nb, y, bf);
-  }
+  lora_expand_all<kLargeMt, kLargeKb, WIDE>(a, B, rank, frag, t, nb0, kLoraWarps, end, y, bf);
 }
 
 // One CTA: tokens counted per adapter (bucket L: none), buckets cut into
-// items of TM tokens.  items: the count, then {adapter, first place of
-// `order`, tokens} each.  The order inside a bucket does not matter: a
-// token's sums are the same whichever row of an item it takes.
+// items of kLargeTm tokens; the items behind the last get no tokens.  The
+// order inside a bucket does not matter: a token's sums are the same
+// whichever row of an item it takes.
 constexpr int kGroupThreads = 1024;
 
-__global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArgs a, int tm, int32_t* __restrict__ place,
+constexpr int kGroupBatch = 8;   // tokens of a thread whose loads are in flight together
+
+__global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArgs a, int32_t* __restrict__ place,
                                                                    int32_t* __restrict__ order,
-                                                                   int32_t* __restrict__ items) {
+                                                                   int4* __restrict__ items, int max_items) {
   chain_begin();
-  extern __shared__ int s_cnt[];                 // [L+1] tokens, then first place; [L+2] first item
+  constexpr int tm = kLargeTm;
+  extern __shared__ int s_cnt[];                 // [L+1] tokens, then first place; [L+1] first item
   int* s_first = s_cnt + a.L + 1;
   __shared__ int2 s_warp[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -463,16 +533,25 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
   const int64_t T = a.T;
   for (int i = tid; i < buckets; i += kGroupThreads) s_cnt[i] = 0;
   __syncthreads();
-  for (int64_t t0 = 0; t0 < T; t0 += kGroupThreads) {
-    const int64_t t = t0 + tid;
-    const bool in = t < T;
-    const int e = in ? lora_id(a, t) : -2, b = e == -1 ? a.L : e;
-    const uint32_t same = __match_any_sync(0xFFFFFFFFu, b);
-    int base = 0;
-    const int first = __ffs(same) - 1;
-    if (in && lane == first) base = atomicAdd(&s_cnt[b], __popc(same));
-    base = __shfl_sync(0xFFFFFFFFu, base, first);
-    if (in) place[t] = base + __popc(same & ((1u << lane) - 1u));
+  for (int64_t t0 = tid; t0 - tid < T; t0 += kGroupBatch * kGroupThreads) {
+    int b[kGroupBatch];   // -2: no token
+#pragma unroll
+    for (int u = 0; u < kGroupBatch; ++u) {
+      const int64_t t = t0 + u * kGroupThreads;
+      b[u] = t < T ? lora_id(a, t) : -2;
+    }
+#pragma unroll
+    for (int u = 0; u < kGroupBatch; ++u) {
+      const int64_t t = t0 + u * kGroupThreads;
+      if (t - tid >= T) break;   // the whole CTA
+      const int bucket = b[u] == -1 ? a.L : b[u];
+      const uint32_t same = __match_any_sync(0xFFFFFFFFu, bucket);
+      const int first = __ffs(same) - 1;
+      int base = 0;
+      if (bucket >= 0 && lane == first) base = atomicAdd(&s_cnt[bucket], __popc(same));
+      base = __shfl_sync(0xFFFFFFFFu, base, first);
+      if (t < T) place[t] = base + __popc(same & ((1u << lane) - 1u));
+    }
   }
   __syncthreads();
   // exclusive scans of tokens and items over the buckets
@@ -506,23 +585,34 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
     at.x += n;
     at.y += (n + tm - 1) / tm;
   }
-  if (tid == 0) items[0] = total, s_first[buckets] = total;
   __syncthreads();
-  for (int64_t t = tid; t < T; t += kGroupThreads) {
-    const int e = lora_id(a, t);
-    order[s_cnt[e < 0 ? a.L : e] + place[t]] = int32_t(t);
-  }
-  for (int i = tid; i < total; i += kGroupThreads) {
-    int lo = 0, hi = buckets;   // the last bucket with s_first <= i: the one that holds item i
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (s_first[m] <= i) lo = m; else hi = m;
+  for (int64_t t0 = tid; t0 < T; t0 += kGroupBatch * kGroupThreads) {
+    int b[kGroupBatch], at_place[kGroupBatch];
+#pragma unroll
+    for (int u = 0; u < kGroupBatch; ++u) {
+      const int64_t t = t0 + u * kGroupThreads;
+      b[u] = t < T ? lora_id(a, t) : 0;
+      at_place[u] = t < T ? place[t] : 0;
     }
-    const int begin = s_cnt[lo] + (i - s_first[lo]) * tm;
-    const int end = lo + 1 < buckets ? s_cnt[lo + 1] : int(T);
-    items[1 + 3 * i] = lo == a.L ? -1 : lo;
-    items[2 + 3 * i] = begin;
-    items[3 + 3 * i] = min(tm, end - begin);
+#pragma unroll
+    for (int u = 0; u < kGroupBatch; ++u) {
+      const int64_t t = t0 + u * kGroupThreads;
+      if (t < T) order[s_cnt[b[u] < 0 ? a.L : b[u]] + at_place[u]] = int32_t(t);
+    }
+  }
+  for (int i = tid; i < max_items; i += kGroupThreads) {
+    int4 it = make_int4(-1, 0, 0, 0);
+    if (i < total) {
+      int lo = 0, hi = buckets;   // the last bucket with s_first <= i: the one that holds item i
+      while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (s_first[m] <= i) lo = m; else hi = m;
+      }
+      const int begin = s_cnt[lo] + (i - s_first[lo]) * tm;
+      const int end = lo + 1 < buckets ? s_cnt[lo + 1] : int(T);
+      it = make_int4(lo == a.L ? -1 : lo, begin, min(tm, end - begin), lora_rank(a, lo == a.L ? -1 : lo));
+    }
+    items[i] = it;
   }
 }
 
@@ -542,7 +632,7 @@ static LoraSpace lora_space(int64_t T, int L, int R) {
   LoraSpace s;
   s.place = up(4 * T);
   s.items = s.place + up(4 * T);
-  s.h = s.items + up(4 * (1 + 3 * lora_max_items(T, L, kLargeTm)));
+  s.h = s.items + up(16 * lora_max_items(T, L, kLargeTm));
   s.bytes = s.h + T * ((R + 15) / 16 * 64);
   return s;
 }
@@ -557,12 +647,12 @@ static cudaError_t launch_lora_small(const LoraArgs& a, cudaStream_t st) {
   while (C > 1 && n * C > 4 * int64_t(sm_count())) C /= 2;
   auto k = lora_small_kernel<WIDE>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), lora_small_smem(kLoraMaxRank), done);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), lora_small_smem(kLoraMaxRank, 8), done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(n * C));
   cfg.blockDim = dim3(kLoraThreads);
-  cfg.dynamicSmemBytes = size_t(lora_small_smem(a.R));
+  cfg.dynamicSmemBytes = size_t(lora_small_smem(a.R, C));
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -578,24 +668,25 @@ static cudaError_t launch_lora_small(const LoraArgs& a, cudaStream_t st) {
 template <bool WIDE>
 static cudaError_t launch_lora_large(const LoraArgs& a, char* ws, cudaStream_t st) {
   const LoraSpace sp = lora_space(a.T, a.L, a.R);
-  int32_t *order = reinterpret_cast<int32_t*>(ws), *place = reinterpret_cast<int32_t*>(ws + sp.place),
-          *items = reinterpret_cast<int32_t*>(ws + sp.items);
+  int32_t *order = reinterpret_cast<int32_t*>(ws), *place = reinterpret_cast<int32_t*>(ws + sp.place);
+  int4* items = reinterpret_cast<int4*>(ws + sp.items);
   uint16_t* h = reinterpret_cast<uint16_t*>(ws + sp.h);
   const unsigned n = unsigned(lora_max_items(a.T, a.L, kLargeTm));
-  static std::atomic<uint64_t> done1{0}, done2{0};
+  // outputs of an expanding CTA: 1,024 spread its start over more blocks (8,192
+  // tokens x 4,096 outputs 54 against 56 us) while that leaves a CTA for every
+  // SM; else 512 (512 tokens: 22 against 24 us)
+  const int cols = int64_t(n) * ((a.N + 1023) / 1024) >= 2 * sm_count() ? 1024 : 512;
+  static std::atomic<uint64_t> done{0};
   auto expand = lora_expand_kernel<WIDE>;
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(lora_shrink_kernel), lora_shrink_smem(kLoraMaxRank), done1);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(expand), lora_frag_bytes(kLargeMt, kLoraMaxRank), done);
   if (e == cudaSuccess)
-    e = allow_smem(reinterpret_cast<const void*>(expand), lora_frag_bytes(kLargeMt, kLoraMaxRank), done2);
+    e = launch_chained(lora_group_kernel, dim3(1), dim3(kGroupThreads), size_t(2 * a.L + 2) * sizeof(int), st, a,
+                       place, order, items, int(n));
   if (e == cudaSuccess)
-    e = launch_chained(lora_group_kernel, dim3(1), dim3(kGroupThreads), size_t(2 * a.L + 3) * sizeof(int), st, a,
-                       kLargeTm, place, order, items);
+    e = launch_chained(lora_shrink_kernel, dim3(n), dim3(kLoraThreads), 0, st, a, order, items, h);
   if (e == cudaSuccess)
-    e = launch_chained(lora_shrink_kernel, dim3(n), dim3(kLoraThreads), size_t(lora_shrink_smem(a.R)), st, a, order,
-                       items, h);
-  if (e == cudaSuccess)
-    e = launch_chained(expand, dim3(n, unsigned((a.N + kExpandCols - 1) / kExpandCols)), dim3(kLoraThreads),
-                       size_t(lora_frag_bytes(kLargeMt, a.R)), st, a, order, items, h);
+    e = launch_chained(expand, dim3(n, unsigned((a.N + cols - 1) / cols)), dim3(kLoraThreads),
+                       size_t(lora_frag_bytes(kLargeMt, a.R)), st, a, order, items, h, cols);
   return e;
 }
 
@@ -604,7 +695,7 @@ cudaError_t launch_lora(const LoraArgs& a, void* workspace, cudaStream_t st) {
   auto aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
   const bool wide = a.N % 8 == 0 && aligned(a.y, a.T > 1 ? a.ldy : 0) && aligned(a.out, a.T > 1 ? a.ldo : 0);
   if (a.T <= kLoraSmall) return wide ? launch_lora_small<true>(a, st) : launch_lora_small<false>(a, st);
-  if ((a.N + kExpandCols - 1) / kExpandCols > 65535) return cudaErrorInvalidValue;
+  if (a.N > 512 * 65535) return cudaErrorInvalidValue;
   char* ws = static_cast<char*>(workspace);
   return wide ? launch_lora_large<true>(a, ws, st) : launch_lora_large<false>(a, ws, st);
 }
