@@ -770,7 +770,7 @@ def _row_view(t: torch.Tensor, name: str, dtype: torch.dtype, align: int = 1):
         raise TypeError(f"{name} must be a torch tensor")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on a CUDA device (no CPU path)")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
     if t.dim() != 2:
         if t.dim() < 1 or t.shape[-1] == 0:
@@ -779,18 +779,17 @@ def _row_view(t: torch.Tensor, name: str, dtype: torch.dtype, align: int = 1):
     n, d = t.shape
     if d == 0:
         raise ValueError(f"{name} must have shape [..., width], got {tuple(t.shape)}")
-    ld = t.stride(0) if n > 1 else d
-    if (t.stride(1) != 1 and d > 1) or ld < d:
+    s0, s1 = t.stride()
+    ld = s0 if n > 1 else d
+    if (s1 != 1 and d > 1) or ld < d:
         t, ld = t.contiguous(), d
     if align > 1 and (t.data_ptr() % align or ld * t.element_size() % align):
         t, ld = t.clone(memory_format=torch.contiguous_format), d
     return t, ld
 
 
-def _same_device(dev: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, x on {dev}")
+def _other_device(name: str, t: torch.Tensor, dev: torch.device) -> ValueError:
+    return ValueError(f"{name} is on {t.device}, x on {dev}")
 
 
 def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tuple) -> Optional[torch.Tensor]:
@@ -798,15 +797,15 @@ def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tup
     if t is None:
         return None
     _require_cuda(t, name)
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     return t.contiguous()
 
 
 def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
-    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
     return _i32(t, dev, name)
 
@@ -821,14 +820,6 @@ def _call(dev: torch.device, what: str, fn, *args) -> None:
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, what)
-
-
-def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A new contiguous tensor of t's shape (empty_like is the cheapest call
-    that allocates, and keeps strides only where they are not contiguous)."""
-    if t.is_contiguous():
-        return torch.empty_like(t, dtype=dtype)
-    return torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 class AddNorm(NamedTuple):
@@ -856,23 +847,29 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
     gain = _bf16(gain, "gain")
     if gain.numel() != d:
         raise ValueError("gain must have the hidden size")
-    _same_device(dev, residual=residual, gain=gain)
+    if gain.device != dev:
+        raise _other_device("gain", gain, dev)
     shape = x.shape
+    # empty_like is the cheapest call that allocates; it keeps strides, so it
+    # takes a contiguous tensor
+    like = x if x.is_contiguous() else torch.empty(shape, dtype=torch.bfloat16, device=dev)
     res_out = r2 = None
     ldr, res_type = 0, _lib.VX_DTYPE_BF16
     if residual is not None:
-        if residual.dtype == torch.float32:
+        if residual.dtype is torch.float32:
             res_type = _lib.VX_DTYPE_F32
-        elif residual.dtype != torch.bfloat16:
+        elif residual.dtype is not torch.bfloat16:
             raise TypeError(f"residual must be bfloat16 or float32, got {residual.dtype}")
         if residual.shape != shape:
             raise ValueError(f"residual shape {tuple(residual.shape)} != {tuple(shape)}")
+        if residual.device != dev:
+            raise _other_device("residual", residual, dev)
         r2, ldr = _row_view(residual, "residual", residual.dtype)
-        res_out = _like(x, residual.dtype)
-    y = _like(x, torch.bfloat16) if output != "e4m3" else None
+        res_out = torch.empty_like(like, dtype=residual.dtype)
+    y = torch.empty_like(like) if output != "e4m3" else None
     q = scales = None
     if output != "bf16":
-        q = _like(x, torch.float8_e4m3fn)
+        q = torch.empty_like(like, dtype=torch.float8_e4m3fn)
         scales = x2.new_empty(shape[:-1], dtype=torch.float32)
     _call(dev, "add_rms_norm", _lib.load().vx_add_rmsnorm, x2.data_ptr(), ldx, _ptr(r2), res_type, ldr,
           gain.data_ptr(), T, d, float(eps), _ptr(res_out), _ptr(y), _ptr(q), _ptr(scales))
@@ -894,9 +891,10 @@ def swiglu_e4m3(gate: torch.Tensor, up: torch.Tensor) -> E4M3Rows:
     if gate.shape != up.shape:
         raise ValueError("gate and up must have the same shape")
     dev = g2.device
-    _same_device(dev, up=u2)
+    if u2.device != dev:
+        raise _other_device("up", u2, dev)
     rows, width = g2.shape
-    q = _like(gate, torch.float8_e4m3fn)
+    q = gate.new_empty(gate.shape, dtype=torch.float8_e4m3fn)
     scales = g2.new_empty(gate.shape[:-1], dtype=torch.float32)
     _call(dev, "swiglu_e4m3", _lib.load().vx_swiglu_e4m3, g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width,
           q.data_ptr(), scales.data_ptr())
@@ -918,7 +916,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     bf16 [P, N], P the length of ``rows`` (or M); positions from
     ``offsets[E]`` on are left as they were in ``out`` (undefined when it is
     allocated here).  K must be a multiple of 16 bytes."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+    e4m3 = isinstance(x, torch.Tensor) and x.dtype is torch.float8_e4m3fn
+    if not e4m3 and not (isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16):
         raise TypeError("x must be a bfloat16 or float8_e4m3fn tensor")
     if x.dim() != 2:
         raise ValueError(f"x must have shape [rows, K], got {tuple(x.shape)}")
@@ -928,15 +927,16 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     _require_cuda(w, "w")
     if w.dtype != x.dtype:
         raise TypeError(f"w must be {str(x.dtype)[6:]} as x, got {w.dtype}")
-    if w.dim() != 3 or w.shape[2] != K or 0 in w.shape or not w.is_contiguous():
+    if w.dim() != 3 or w.shape[2] != K or not w.numel() or not w.is_contiguous():
         raise ValueError(f"w must be a contiguous [experts, out, {K}], got {tuple(w.shape)}")
     if w.data_ptr() % 16 or K * w.element_size() % 16:
         raise ValueError("w must start on a 16-byte boundary and its rows be multiples of 16 bytes")
-    E, N = int(w.shape[0]), int(w.shape[1])
-    e4m3 = x.dtype == torch.float8_e4m3fn
+    E, N, _ = w.shape
     if e4m3 != (x_scales is not None) or e4m3 != (w_scales is not None):
         raise ValueError("float8_e4m3fn takes x_scales and w_scales, bfloat16 neither")
-    _same_device(dev, w=w, x_scales=x_scales, w_scales=w_scales, out=out)
+    for name, t in (("w", w), ("x_scales", x_scales), ("w_scales", w_scales), ("out", out)):
+        if t is not None and t.device != dev:
+            raise _other_device(name, t, dev)
     x_scales = _vector(x_scales, "x_scales", torch.float32, (M,))
     w_scales = _vector(w_scales, "w_scales", torch.float32, (E, N))
     offsets = _ids(offsets, "offsets", dev)
@@ -944,7 +944,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
         raise ValueError(f"offsets must hold {E + 1} values, got {offsets.numel()}")
     P = M
     if rows is not None:
-        rows = _ids(rows, "rows", dev).reshape(-1)
+        rows = _ids(rows, "rows", dev)
         P = rows.numel()
     elif slots != 1:
         raise ValueError("slots needs rows")
@@ -988,10 +988,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     _require_cuda(b, "b")
     if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
         raise TypeError(f"a and b must be bfloat16, got {a.dtype} and {b.dtype}")
-    if a.dim() != 3 or 0 in a.shape or a.shape[2] != K or not a.is_contiguous():
+    if a.dim() != 3 or not a.numel() or a.shape[2] != K or not a.is_contiguous():
         raise ValueError(f"a must be a contiguous [adapters, rank, {K}], got {tuple(a.shape)}")
-    L, R = int(a.shape[0]), int(a.shape[1])
-    if tuple(b.shape) != (L, N, R) or not b.is_contiguous():
+    L, R, _ = a.shape
+    if b.shape != (L, N, R) or not b.is_contiguous():
         raise ValueError(f"b must be a contiguous {(L, N, R)}, got {tuple(b.shape)}")
     if K % 8 or R % 8 or R > 256 or L > 4096:
         raise ValueError(f"K {K} and rank {R} must be multiples of 8, the rank at most 256, adapters ({L}) 4096")
@@ -999,14 +999,16 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         raise ValueError("a and b must start on 16-byte boundaries")
     if x.shape[:-1] != y.shape[:-1]:
         raise ValueError(f"x and y rows differ: {tuple(x.shape[:-1])} and {tuple(y.shape[:-1])}")
-    _same_device(dev, y=y2, a=a, b=b, scales=scales, ranks=ranks, out=out)
+    for name, t in (("y", y2), ("a", a), ("b", b), ("scales", scales), ("ranks", ranks), ("out", out)):
+        if t is not None and t.device != dev:
+            raise _other_device(name, t, dev)
     adapters = _ids(adapters, "adapters", dev)
     if adapters.numel() != T:
         raise ValueError(f"adapters must name one adapter a row ({T}), got {adapters.numel()}")
     scales = _vector(scales, "scales", torch.float32, (L,))
     ranks = _vector(ranks, "ranks", torch.int32, (L,))
     if out is None:
-        out = _like(y, torch.bfloat16)
+        out = torch.empty_like(y) if y.is_contiguous() else y.new_empty(y.shape)
         ldo = N
     else:
         o2, ldo = _row_view(out, "out", torch.bfloat16)
