@@ -373,12 +373,15 @@ int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_
  * over T * slots routed ids: a position reads its token's row of x.
  * Positions from offsets[experts] on are left as they were; a position whose
  * row lies outside [0, x_rows) gets zeros; offsets are clamped to
- * [0, P] and to ascend.  K and ldx are multiples of 16 bytes, x and w start
- * on 16-byte boundaries. */
+ * [0, P] and to ascend.  At most 2048 experts; K and ldx are multiples of 16
+ * bytes, x and w start on 16-byte boundaries.  The workspace (16-byte aligned) is needed for
+ * larger batches with rows (vx_grouped_matmul_workspace is 0 else). */
+size_t vx_grouped_matmul_workspace(int32_t dtype, int64_t P, int32_t experts, int32_t K, int32_t with_rows);
 int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx, const void* w,
                       const float* x_scales, const float* w_scales, const int32_t* offsets,
                       int32_t experts, int32_t N, int32_t K, const int32_t* rows, int32_t slots,
-                      int64_t P, uint16_t* out, int64_t ldo, void* stream);
+                      int64_t P, uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 /* Low-rank adapters of many requests beside a shared projection whose output
  * is y: out[t, :] = y[t, :] + scales[e] * b[e] (a[e] x[t, :]) with e =

@@ -48,12 +48,12 @@ def test_grouped_matmul_refusals(lib):
     from vxmoe import _lib
 
     def call(x=P16, dtype=0, x_rows=8, ldx=64, w=P16, xs=None, ws=None, offsets=P16, E=4, N=24, K=64, rows=None,
-             slots=1, P=8, out=P16, ldo=24):
+             slots=1, P=8, out=P16, ldo=24, space=None, nbytes=0):
         return lib.vx_grouped_matmul(x, dtype, x_rows, ldx, w, xs, ws, offsets, E, N, K, rows, slots, P, out, ldo,
-                                     None)
+                                     space, nbytes, None)
 
     e4m3 = dict(dtype=2, xs=P16, ws=P16)
-    for kw in (dict(E=0), dict(E=4097), dict(N=0), dict(K=0), dict(K=4, ldx=8), dict(ldx=60), dict(ldx=68),
+    for kw in (dict(E=0), dict(E=2049), dict(N=0), dict(K=0), dict(K=4, ldx=8), dict(ldx=60), dict(ldx=68),
                dict(slots=0), dict(P=-1), dict(P=1 << 31), dict(x_rows=1 << 31, P=1), dict(x_rows=-1),
                dict(x_rows=7), dict(slots=2), dict(ldo=23), dict(xs=P16), dict(ws=P16), dict(dtype=2),
                dict(dtype=2, xs=P16), dict(K=56, ldx=64, **e4m3), dict(K=48, ldx=56, **e4m3), dict(x=None),
@@ -62,6 +62,14 @@ def test_grouped_matmul_refusals(lib):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw
     assert call(dtype=1) == _lib.VX_EINVAL_DTYPE
     assert call(P=0, x=None, x_rows=0, offsets=None, out=None) == _lib.VX_OK
+    assert lib.vx_grouped_matmul_workspace(0, 100000, 4, 64, 0) == 0
+    assert lib.vx_grouped_matmul_workspace(0, 8, 4, 64, 1) == 0
+    need = lib.vx_grouped_matmul_workspace(0, 100000, 4, 64, 1)
+    assert need >= 100000 * 128 and lib.vx_grouped_matmul_workspace(2, 100000, 4, 64, 1) >= 100000 * 68
+    for kw in (dict(), dict(space=P16, nbytes=need - 1), dict(space=ODD, nbytes=need)):
+        assert call(P=100000, rows=P16, **kw) == _lib.VX_EWORKSPACE, kw
+    assert lib.vx_grouped_matmul_workspace(1, 100000, 4, 64, 1) == 0
+    assert lib.vx_grouped_matmul_workspace(0, -1, 4, 64, 1) == lib.vx_grouped_matmul_workspace(0, 1, 0, 64, 1) == 0
 
 
 def test_lora_add_refusals(lib):

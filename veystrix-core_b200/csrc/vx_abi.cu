@@ -1109,10 +1109,16 @@ int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 
+size_t vx_grouped_matmul_workspace(int32_t dtype, int64_t P, int32_t experts, int32_t K, int32_t with_rows) {
+  if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return 0;
+  if (P < 0 || P > 0x7FFF0000 || experts < 1 || experts > kGroupedMaxExperts || K < 1) return 0;
+  return size_t(grouped_workspace_bytes(P, experts, K, dtype == VX_DTYPE_E4M3, with_rows != 0));
+}
+
 int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx, const void* w,
                       const float* x_scales, const float* w_scales, const int32_t* offsets, int32_t experts,
                       int32_t N, int32_t K, const int32_t* rows, int32_t slots, int64_t P, uint16_t* out,
-                      int64_t ldo, void* stream) {
+                      int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return VX_EINVAL_DTYPE;
   const int size = dtype == VX_DTYPE_BF16 ? 2 : 1;
   if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1) return VX_EINVAL_SHAPE;
@@ -1124,8 +1130,10 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
   if (P == 0) return VX_OK;   // empty tensors may come as null pointers
   if (dtype == VX_DTYPE_BF16 ? (x_scales || w_scales) : (!x_scales || !w_scales)) return VX_EINVAL_SHAPE;
   if (!x || !w || !offsets || !out || x_rows < 1 || !aligned16(x) || !aligned16(w)) return VX_EINVAL_SHAPE;
+  const size_t need = vx_grouped_matmul_workspace(dtype, P, experts, K, rows != nullptr);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return VX_EWORKSPACE;
   GroupedArgs a{x, x_rows, ldx, w, x_scales, w_scales, offsets, experts, N, K, rows, slots, P, out, ldo};
-  cudaError_t e = launch_grouped(a, dtype == VX_DTYPE_E4M3, static_cast<cudaStream_t>(stream));
+  cudaError_t e = launch_grouped(a, dtype == VX_DTYPE_E4M3, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? VX_OK : vx_cuda_fail(e);
 }
 

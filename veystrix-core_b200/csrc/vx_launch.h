@@ -372,7 +372,7 @@ cudaError_t launch_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t
                                int width, uint8_t* q, float* scales, cudaStream_t st);
 
 // Products grouped by expert over bf16 or e4m3 banks (vx_grouped.cu).
-constexpr int kGroupedMaxExperts = 4096;
+constexpr int kGroupedMaxExperts = 2048;
 struct GroupedArgs {
   const void* x;                // [x_rows][ldx]
   int64_t x_rows, ldx;
@@ -387,7 +387,8 @@ struct GroupedArgs {
   uint16_t* out;                // [P][ldo]
   int64_t ldo;
 };
-cudaError_t launch_grouped(const GroupedArgs& a, bool e4m3, cudaStream_t st);
+int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows);   // 0: none
+cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st);
 
 // Low-rank adapters (vx_lora.cu).
 constexpr int kLoraMaxRank = 256;

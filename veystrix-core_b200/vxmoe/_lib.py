@@ -131,7 +131,8 @@ SIGNATURES = {
                                       P]),
     "vx_swiglu_e4m3": (ctypes.c_int, [P, c_int64, P, c_int64, c_int64, c_int32, P, P, P]),
     "vx_grouped_matmul": (ctypes.c_int, [P, c_int32, c_int64, c_int64, P, P, P, P, c_int32, c_int32, c_int32, P,
-                                         c_int32, c_int64, P, c_int64, P]),
+                                         c_int32, c_int64, P, c_int64, P, c_size_t, P]),
+    "vx_grouped_matmul_workspace": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
     "vx_lora_add": (ctypes.c_int, [P, c_int64, P, c_int64, P, P, P, P, P, c_int32, c_int64, c_int32, c_int32,
                                    c_int32, P, c_int64, P, c_size_t, P]),
     "vx_lora_add_workspace": (c_size_t, [c_int64, c_int32, c_int32]),

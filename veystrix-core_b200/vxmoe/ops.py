@@ -894,7 +894,8 @@ def swiglu_e4m3(gate: torch.Tensor, up: torch.Tensor) -> E4M3Rows:
     if u2.device != dev:
         raise _other_device("up", u2, dev)
     rows, width = g2.shape
-    q = gate.new_empty(gate.shape, dtype=torch.float8_e4m3fn)
+    q = (torch.empty_like(gate, dtype=torch.float8_e4m3fn) if gate.is_contiguous()
+         else gate.new_empty(gate.shape, dtype=torch.float8_e4m3fn))
     scales = g2.new_empty(gate.shape[:-1], dtype=torch.float32)
     _call(dev, "swiglu_e4m3", _lib.load().vx_swiglu_e4m3, g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width,
           q.data_ptr(), scales.data_ptr())
@@ -932,6 +933,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     if w.data_ptr() % 16 or K * w.element_size() % 16:
         raise ValueError("w must start on a 16-byte boundary and its rows be multiples of 16 bytes")
     E, N, _ = w.shape
+    if E > 2048:
+        raise ValueError(f"at most 2048 experts, got {E}")
     if e4m3 != (x_scales is not None) or e4m3 != (w_scales is not None):
         raise ValueError("float8_e4m3fn takes x_scales and w_scales, bfloat16 neither")
     for name, t in (("w", w), ("x_scales", x_scales), ("w_scales", w_scales), ("out", out)):
@@ -960,10 +963,14 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
             raise ValueError(f"out must be rows of shape {(P, N)}, got {tuple(out.shape)}")
     if P and not M:
         raise ValueError("rows need rows of x")
-    _call(dev, "grouped_matmul", _lib.load().vx_grouped_matmul, x.data_ptr(),
-          _lib.VX_DTYPE_E4M3 if e4m3 else _lib.VX_DTYPE_BF16, M, ldx, w.data_ptr(), _ptr(x_scales), _ptr(w_scales),
+    lib = _lib.load()
+    kind = _lib.VX_DTYPE_E4M3 if e4m3 else _lib.VX_DTYPE_BF16
+    nbytes = lib.vx_grouped_matmul_workspace(kind, P, E, K, 1) if rows is not None else 0
+    # its own allocation: a captured graph keeps it in its own pool
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, "grouped_matmul", lib.vx_grouped_matmul, x.data_ptr(), kind, M, ldx, w.data_ptr(), _ptr(x_scales), _ptr(w_scales),
           offsets.data_ptr(), E, N, K, _ptr(rows), int(slots), P, out.data_ptr(),
-          out.stride(0) if P > 1 else N)
+          out.stride(0) if P > 1 else N, _ptr(ws), nbytes)
     return out
 
 
