@@ -301,13 +301,23 @@ VX_DEVICE void lora_expand(const LoraArgs& a, const uint16_t* B, int rank, const
     store8<WIDE>(a.out + t[i] * a.ldo, n, a.N, v);
   }
 }
-// The 32-output blocks first, first + stride, ... below `end`, each one's y
-// and B loaded before its predecessor is computed; the first block's are
-// loaded by the caller.
-template <int MT, int KB, bool WIDE>
+// The 32-output blocks first, first + stride, ... below `end`; the first
+// block's y and B are loaded by the caller.  AHEAD: each block's are loaded
+// before its predecessor is computed.
+template <int MT, int KB, bool WIDE, bool AHEAD>
 VX_DEVICE void lora_expand_all(const LoraArgs& a, const uint16_t* B, int rank, const uint4* frag,
                                const int (&t)[2 * MT], int first, int stride, int end, Eight<WIDE> (&y)[2 * MT],
                                uint4 (&bf)[KB][4]) {
+  if constexpr (!AHEAD) {
+    for (int nb = first; nb * 32 < end; nb += stride) {
+      if (nb != first) {
+        load_b<KB>(a, B, rank, nb, 0, bf);
+        load_y<MT, WIDE>(a, t, nb, y);
+      }
+      lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, y, bf);
+    }
+    return;
+  }
   Eight<WIDE> yn[2 * MT];
   uint4 bn[KB][4];
   int nb = first;
@@ -426,7 +436,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
     }
     __syncthreads();
   }
-  lora_expand_all<1, kSmallKb, WIDE>(a, B, rank, frag, t, nb0, stride, a.N, y, bf);
+  lora_expand_all<1, kSmallKb, WIDE, true>(a, B, rank, frag, t, nb0, stride, a.N, y, bf);
 }
 
 // ---- large batches ------------------------------------------------------------
@@ -509,7 +519,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
     p[2] = v.y;   // 2, 3: two registers on
   }
   __syncthreads();
-  lora_expand_all<kLargeMt, kLargeKb, WIDE>(a, B, rank, frag, t, nb0, kLoraWarps, end, y, bf);
+  lora_expand_all<kLargeMt, kLargeKb, WIDE, true>(a, B, rank, frag, t, nb0, kLoraWarps, end, y, bf);
 }
 
 // One CTA: tokens counted per adapter (bucket L: none), buckets cut into
@@ -530,27 +540,34 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
   __shared__ int2 s_warp[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int buckets = a.L + 1;
-  const int64_t T = a.T;
-  for (int i = tid; i < buckets; i += kGroupThreads) s_cnt[i] = 0;
-  __syncthreads();
-  for (int64_t t0 = tid; t0 - tid < T; t0 += kGroupBatch * kGroupThreads) {
-    int b[kGroupBatch];   // -2: no token
+  const int64_t T = a.T, round = int64_t(kGroupBatch) * kGroupThreads;
+  int b[kGroupBatch], at[kGroupBatch];           // buckets (-1: no token) and places of a round's tokens
+  auto load = [&](int64_t t0) {
 #pragma unroll
     for (int u = 0; u < kGroupBatch; ++u) {
       const int64_t t = t0 + u * kGroupThreads;
       b[u] = t < T ? lora_id(a, t) : -2;
     }
 #pragma unroll
+    for (int u = 0; u < kGroupBatch; ++u) b[u] = b[u] == -1 ? a.L : b[u] == -2 ? -1 : b[u];
+  };
+  load(tid);
+  for (int i = tid; i < buckets; i += kGroupThreads) s_cnt[i] = 0;
+  __syncthreads();
+  for (int64_t r0 = 0; r0 < T; r0 += round) {
+    if (r0 > 0) load(r0 + tid);
+#pragma unroll
     for (int u = 0; u < kGroupBatch; ++u) {
-      const int64_t t = t0 + u * kGroupThreads;
-      if (t - tid >= T) break;   // the whole CTA
-      const int bucket = b[u] == -1 ? a.L : b[u];
-      const uint32_t same = __match_any_sync(0xFFFFFFFFu, bucket);
-      const int first = __ffs(same) - 1;
-      int base = 0;
-      if (bucket >= 0 && lane == first) base = atomicAdd(&s_cnt[bucket], __popc(same));
-      base = __shfl_sync(0xFFFFFFFFu, base, first);
-      if (t < T) place[t] = base + __popc(same & ((1u << lane) - 1u));
+      if (r0 + u * kGroupThreads >= T) break;   // the whole CTA
+      // a warp of one bucket (packed prompts) adds once, others lane by lane
+      if (__all_sync(0xFFFFFFFFu, b[u] == __shfl_sync(0xFFFFFFFFu, b[u], 0))) {
+        int base = 0;
+        if (lane == 0 && b[u] >= 0) base = atomicAdd(&s_cnt[b[u]], 32);
+        at[u] = __shfl_sync(0xFFFFFFFFu, base, 0) + lane;
+      } else if (b[u] >= 0) {
+        at[u] = atomicAdd(&s_cnt[b[u]], 1);
+      }
+      if (T > round && b[u] >= 0) place[r0 + u * kGroupThreads + tid] = at[u];
     }
   }
   __syncthreads();
@@ -558,7 +575,7 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
   const int per = (buckets + kGroupThreads - 1) / kGroupThreads;
   int2 own = make_int2(0, 0);
   for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i, n = b < buckets ? s_cnt[b] : 0;
+    const int bucket = tid * per + i, n = bucket < buckets ? s_cnt[bucket] : 0;
     own.x += n;
     own.y += (n + tm - 1) / tm;
   }
@@ -570,34 +587,35 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
   }
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  int2 at = make_int2(inc.x - own.x, inc.y - own.y);
+  int2 next = make_int2(inc.x - own.x, inc.y - own.y);
   int total = 0;
   for (int w = 0; w < 32; ++w) {
-    if (w < warp) at.x += s_warp[w].x, at.y += s_warp[w].y;
+    if (w < warp) next.x += s_warp[w].x, next.y += s_warp[w].y;
     total += s_warp[w].y;
   }
   for (int i = 0; i < per; ++i) {
-    const int b = tid * per + i;
-    if (b >= buckets) break;
-    const int n = s_cnt[b];
-    s_cnt[b] = at.x;
-    s_first[b] = at.y;
-    at.x += n;
-    at.y += (n + tm - 1) / tm;
+    const int bucket = tid * per + i;
+    if (bucket >= buckets) break;
+    const int n = s_cnt[bucket];
+    s_cnt[bucket] = next.x;
+    s_first[bucket] = next.y;
+    next.x += n;
+    next.y += (n + tm - 1) / tm;
   }
   __syncthreads();
-  for (int64_t t0 = tid; t0 < T; t0 += kGroupBatch * kGroupThreads) {
-    int b[kGroupBatch], at_place[kGroupBatch];
+  for (int64_t r0 = 0; r0 < T; r0 += round) {
+    if (T > round) {   // else still in registers
+      load(r0 + tid);
 #pragma unroll
-    for (int u = 0; u < kGroupBatch; ++u) {
-      const int64_t t = t0 + u * kGroupThreads;
-      b[u] = t < T ? lora_id(a, t) : 0;
-      at_place[u] = t < T ? place[t] : 0;
+      for (int u = 0; u < kGroupBatch; ++u) {
+        const int64_t t = r0 + u * kGroupThreads + tid;
+        at[u] = t < T ? place[t] : 0;
+      }
     }
 #pragma unroll
     for (int u = 0; u < kGroupBatch; ++u) {
-      const int64_t t = t0 + u * kGroupThreads;
-      if (t < T) order[s_cnt[b[u] < 0 ? a.L : b[u]] + at_place[u]] = int32_t(t);
+      const int64_t t = r0 + u * kGroupThreads + tid;
+      if (t < T) order[s_cnt[b[u]] + at[u]] = int32_t(t);
     }
   }
   for (int i = tid; i < max_items; i += kGroupThreads) {

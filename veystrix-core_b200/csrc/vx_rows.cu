@@ -14,9 +14,8 @@
 // the float32 range take a second one over scaled values, or the values
 // themselves.  Rows are bound by memory: a row's elements
 // are read once, stay in the registers of its threads (as float32) until the
-// reduction is done, and every output is written once.  The maximum is taken
-// over the bit patterns of |v|, an order in which NaN is above infinity, so a
-// NaN anywhere makes the row's scale NaN as the formula does.
+// reduction is done, and every output is written once.  The maximum keeps
+// NaN, so a NaN anywhere makes the row's scale NaN as the formula does.
 //
 // Rows are dealt round robin to groups of threads, a warp (four groups a CTA)
 // or a CTA; a group has its next row's loads in flight while it reduces and
@@ -36,8 +35,6 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kScaleMin = 0x1p-126f;
 constexpr float kFloatMax = 0x1.fffffep127f;
 
-VX_DEVICE uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
 // {scale, 1/scale} of a row whose largest |v| is amax (NaN stays NaN).
 VX_DEVICE float2 row_scale(float amax) {
   float s = __fdiv_rn(amax, kE4m3Max);
@@ -54,12 +51,22 @@ VX_DEVICE uint32_t bf16x2(float lo, float hi) {
   return r;
 }
 
-// 1/(1 + exp(-g)): with e = exp(-|g|) <= 1 the denominator stays in [1, 2],
-// where the approximate division is good to 2 ulp, and nothing overflows;
-// the fast exponential is off by |g| 2^-24 of e.
-VX_DEVICE float sigmoid_f32(float g) {
-  const float e = __expf(-fabsf(g));
-  return __fdividef(g < 0.f ? e : 1.0f, 1.0f + e);
+// g / (1 + exp(-g)) * u.  With e = exp(-|g|) <= 1 the denominator stays in
+// [1, 2] and nothing overflows; e is the square of 2^(-|g| log2(e) / 2),
+// which no |g| whose e counts takes out of the normal range, so the
+// flush-to-zero exponential serves (half the instructions of the one that
+// keeps subnormals).  Off by a few 2^-22 and |g| 2^-24 of e.
+VX_DEVICE float swiglu_f32(float g, float u) {
+  float h, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(g) * -0.72134752f));
+  const float e = h * h;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * (g < 0.f ? e : 1.0f) * r * u;
+}
+// The larger of top and |v|, NaN if one of them is.
+VX_DEVICE float max_abs(float top, float v) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(v)));
+  return top;
 }
 
 // V elements of a row as they lie in memory, and as float32.
@@ -130,14 +137,16 @@ VX_DEVICE void store_row(uint8_t* p, const float (&f)[V]) {
     *p = uint8_t(e4m3x2(f[0], 0.f));
 }
 
-// Sum (SUM) and largest bit pattern over the threads of a row: its warp, or
+// Sum (SUM) and largest value over the threads of a row: its warp, or
 // the CTA (ONE_WARP false).  Every thread adds the warps' sums in the same
 // order.  Successive calls alternate `turn` between two sets of shared
 // memory, so one barrier a call is enough.
 template <bool ONE_WARP, bool SUM>
-VX_DEVICE void row_reduce(float& sum, uint32_t& top, int& turn) {
+VX_DEVICE void row_reduce(float& sum, float& largest, int& turn) {
   if (SUM) sum = warp_sum<32>(sum);
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  // not negative: ordered like their bit patterns, NaN on top
+  uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(largest));
+  largest = __uint_as_float(top);
   if (ONE_WARP) return;
   __shared__ float sums[2][32];
   __shared__ uint32_t tops[2][32];
@@ -149,6 +158,7 @@ VX_DEVICE void row_reduce(float& sum, uint32_t& top, int& turn) {
     if (SUM) sum += sums[turn][w];
     top = max(top, tops[turn][w]);
   }
+  largest = __uint_as_float(top);
   turn ^= 1;
 }
 
@@ -210,8 +220,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
   }
   for (int64_t t = grp.row; t < T; t += grp.stride) {   // whole groups
     float s[NV][V];
-    float sum = 0.f;
-    uint32_t top = 0;
+    float sum = 0.f, top = 0.f;   // top: max |s gain|, then max |v|
     // f(s, gain) over the thread's elements
     auto each = [&](auto&& f) {
       if constexpr (LOOP) {
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
     }
     each([&](float sv, float gv) {
       sum = fmaf(sv, sv, sum);
-      top = max(top, abs_bits(sv * gv));
+      top = max_abs(top, sv * gv);
     });
     row_reduce<ONE_WARP, true>(sum, top, turn);
     float r;
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       // the squares left the float32 range: the same on s / 2^70 (both
       // branches are taken by whole rows)
       sum = 0.f;
-      uint32_t unused = 0;
+      float unused = 0.f;
       each([&](float sv, float) {
         sv *= 0x1p-70f;
         sum = fmaf(sv, sv, sum);
@@ -261,16 +270,16 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
     } else {
       r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps)));
     }
-    if (scales && (top >= 0x7F800000u || top < 0x0D800000u)) {
+    if (scales && !(top <= kFloatMax && top >= 0x1p-100f)) {
       // some |s g| is no finite number, or all are below 2^-100 and lose bits:
       // the maximum of the values themselves
-      top = 0;
-      each([&](float sv, float gv) { top = max(top, abs_bits(sv * r * gv)); });
+      top = 0.f;
+      each([&](float sv, float gv) { top = max_abs(top, sv * r * gv); });
       row_reduce<ONE_WARP, false>(sum, top, turn);
     } else {
-      top = __float_as_uint(r * __uint_as_float(top));   // max|v| up to the rounding of one product
+      top *= r;   // max|v| up to the rounding of one product
     }
-    const float2 sc = row_scale(__uint_as_float(top));
+    const float2 sc = row_scale(top);
     if (scales && i0 == 0) scales[t] = sc.x;
 
     auto write = [&](int i, float (&sv)[V]) {
@@ -323,21 +332,20 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) swiglu_e4m3_kernel(
     gw[n].get(o);
     uw[n].get(u);
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = o[j] * sigmoid_f32(o[j]) * u[j];
+    for (int j = 0; j < V; ++j) o[j] = swiglu_f32(o[j], u[j]);
   };
   if (!LOOP && grp.row < rows) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) fetch(grp.row, i0 + n * step, n);
   }
   for (int64_t t = grp.row; t < rows; t += grp.stride) {   // whole groups
-    float v[NV][V], unused = 0.f;
-    uint32_t top = 0;
+    float v[NV][V], unused = 0.f, top = 0.f;
     if constexpr (LOOP) {
       for (int i = i0; i < width; i += step) {
         fetch(t, i, 0);
         value(0, v[0]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[0][j]));
+        for (int j = 0; j < V; ++j) top = max_abs(top, v[0][j]);
       }
     } else {
 #pragma unroll
@@ -349,10 +357,10 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) swiglu_e4m3_kernel(
 #pragma unroll
       for (int n = 0; n < NV; ++n)
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[n][j]));
+        for (int j = 0; j < V; ++j) top = max_abs(top, v[n][j]);
     }
     row_reduce<ONE_WARP, false>(unused, top, turn);
-    const float2 sc = row_scale(__uint_as_float(top));
+    const float2 sc = row_scale(top);
     if (i0 == 0) scales[t] = sc.x;
     auto write = [&](int i, float (&o)[V]) {
 #pragma unroll
