@@ -162,16 +162,38 @@ def test_nothing_to_do():
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
-def test_results_do_not_depend_on_the_batch(kind):
-    """A row's products are the same bits alone and among others, call after call."""
-    x, w, xs, ws = operands(kind, 400, 2, 144, 320)
-    whole = vxmoe.grouped_matmul(x, w, offsets_of([390, 10]), x_scales=xs, w_scales=ws)
-    again = vxmoe.grouped_matmul(x, w, offsets_of([390, 10]), x_scales=xs, w_scales=ws)
+@pytest.mark.parametrize("counts", [[390, 10], [3, 1], [60, 0]])
+def test_calls_repeat_and_rows_do_not_depend_on_their_neighbours(kind, counts):
+    """The same call gives the same bits, whatever the other rows of its groups hold."""
+    x, w, xs, ws = operands(kind, sum(counts), 2, 144, 320)
+    whole = vxmoe.grouped_matmul(x, w, offsets_of(counts), x_scales=xs, w_scales=ws)
+    again = vxmoe.grouped_matmul(x, w, offsets_of(counts), x_scales=xs, w_scales=ws)
     assert torch.equal(whole, again)
-    for i in (0, 200, 389):
-        one = vxmoe.grouped_matmul(x[i:i + 1], w, offsets_of([1, 0]),
-                                   x_scales=None if xs is None else xs[i:i + 1], w_scales=ws)
-        assert torch.equal(one[0], whole[i])
+    other = x.flip(0).contiguous()
+    keep = counts[0] // 2
+    other[keep] = x[keep]
+    if xs is not None:
+        xs = xs.flip(0).contiguous()
+        xs[keep] = operands(kind, sum(counts), 2, 144, 320)[2][keep]
+    mixed = vxmoe.grouped_matmul(other, w, offsets_of(counts), x_scales=xs, w_scales=ws)
+    assert torch.equal(mixed[keep], whole[keep])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("E,P", [(1, 1), (1, 8), (3, 12), (40, 37), (512, 10), (512, 700), (2048, 9)])
+@pytest.mark.parametrize("N,K", [(16, 64), (33, 176), (1000, 2048), (128, 4112)])
+def test_few_rows(kind, E, P, N, K):
+    """Groups around the few-rows kernel's items of 8, one warp and eight to a unit."""
+    if E * N * K > 1 << 28:
+        N = max(1, (1 << 28) // (E * K))
+    x, w, xs, ws = operands(kind, 5, E, N, K, seed=11)
+    ids = torch.randint(0, E, (P,), device="cuda", generator=gen(12))
+    if P > 30:
+        ids[:11] = E // 2          # a group of more than one item
+    ids = ids.sort().values
+    offsets = torch.cat([ids.new_zeros(1), torch.bincount(ids, minlength=E).cumsum(0)]).int()
+    rows = torch.randint(0, 10, (P,), device="cuda", generator=gen(13), dtype=torch.int32)
+    check(x, w, offsets, f"{kind} E={E} P={P} {N}x{K}", rows=rows, slots=2, x_scales=xs, w_scales=ws)
 
 
 def test_two_streams_and_two_graphs_at_once():

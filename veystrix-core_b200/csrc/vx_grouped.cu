@@ -6,7 +6,8 @@
 // rows[p] / slots, or p itself; the scales only with e4m3.  Sums in float32,
 // one rounding.  Positions from offsets[E] on are left as they were.
 //
-// A CTA pair (cluster of two, cta_group::2) computes tiles of 256 outputs x
+// Few rows an expert go to vx_grouped_few.cu.  Here, a CTA pair (cluster of
+// two, cta_group::2) computes tiles of 256 outputs x
 // up to 256 positions of one expert with tcgen05.mma:
 //
 //   D[256 outputs][N positions] += W[256][K] . X[N][K]^T
@@ -55,6 +56,7 @@
 
 #include "vx_async.cuh"
 #include "vx_common.cuh"
+#include "vx_grouped.cuh"
 #include "vx_launch.h"
 #include "vx_tc.cuh"
 
@@ -74,12 +76,6 @@ struct GroupedTc {
   int row_tiles;                                    // 256-output tiles of a bank
   int by_four;                                      // out's rows take 8-byte stores
 };
-
-// The row of x that position p reads; -1 where it lies outside x.
-VX_DEVICE int row_of(const GroupedArgs& a, int p) {
-  const int r = __ldg(a.rows + p);
-  return r >= 0 && r / a.slots < a.x_rows ? r / a.slots : -1;
-}
 
 VX_DEVICE uint32_t cluster_rank() {
   uint32_t r;
@@ -200,15 +196,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   __shared__ __align__(16) int4 row_of_4[2][kGtCols / 2 / 8];   // warps 2, 3: rows of each copy
   __shared__ __align__(16) float x_scale[FP8 ? kGtEpiWarps : 1][kGtCols / 2];   // an epilogue warp's columns
   __shared__ uint32_t tmem_slot;
-  __shared__ int dead, scan[kGtThreads / 32];
+  __shared__ int dead;
   const GroupedArgs& a = g.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  // tiles before expert e, behind the ring
-  int* first_tile = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)) + kGtStages * kGtStage);
-  int* starts = first_tile + a.experts + 1;   // group e: starts[e] .. starts[e + 1] (none if that descends)
-
+  int* table = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)) + kGtStages * kGtStage);
   if (threadIdx.x == 0) {
     dead = 0;
     for (int s = 0; s < kGtStages; ++s) {
@@ -233,39 +226,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   }
   chain_wait();
 
-  // Clamped group starts, and the exclusive scan of the groups' tile counts:
-  // a thread takes neighbouring experts, all its loads at once.
-  {
-    const int P = int(a.P), each = (a.experts + kGtThreads - 1) / kGtThreads, e0 = threadIdx.x * each;
-    auto start = [&](int e) { return min(max(__ldg(a.offsets + e), 0), P); };
-    int v = 0;
-    for (int i = 0, lo = e0 < a.experts ? start(e0) : 0; i < each && e0 + i < a.experts; ++i) {
-      const int hi = start(e0 + i + 1);
-      starts[e0 + i] = lo;
-      first_tile[e0 + i] = v;   // inside the thread's range
-      v += (max(hi - lo, 0) + kGtCols - 1) / kGtCols * g.row_tiles;
-      if (e0 + i + 1 == a.experts) starts[a.experts] = hi;
-      lo = hi;
-    }
-    int up = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xFFFFFFFFu, up, o);
-      if (lane >= o) up += u;
-    }
-    if (lane == 31) scan[warp] = up;
-    __syncthreads();
-    int before = up - v, all = 0;
-#pragma unroll
-    for (int w = 0; w < kGtThreads / 32; ++w) {
-      if (w < warp) before += scan[w];
-      all += scan[w];
-    }
-    for (int i = 0; i < each && e0 + i < a.experts; ++i) first_tile[e0 + i] += before;
-    if (threadIdx.x == 0) first_tile[a.experts] = all;
-  }
-  __syncthreads();
-  const int tiles = first_tile[a.experts];
+  const GroupTable<kGtThreads> groups(a, table, kGtCols);
+  const int tiles = groups.items() * g.row_tiles;
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -273,16 +235,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   auto tile_at = [&](int t) {
-    int lo = 0, hi = a.experts;   // the last e with first_tile[e] <= t
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (first_tile[m] <= t) lo = m; else hi = m;
-    }
-    const int i = t - first_tile[lo], p = starts[lo];
-    const int n = starts[lo + 1] - p, parts = (n + kGtCols - 1) / kGtCols;
-    const int part = i / g.row_tiles, rt = i - part * g.row_tiles;
+    // an expert's tiles: its parts, each with all the row tiles
+    const int part = t / g.row_tiles, rt = t - part * g.row_tiles;
+    const int e = groups.expert(part), n = groups.size(e), parts = (n + kGtCols - 1) / kGtCols;
     const int each = ((n + parts - 1) / parts + 31) & ~31;   // whole MMA steps of 32 columns
-    return Tile{lo, rt * kGtRows, p + part * each, min(each, n - part * each)};
+    const int skip = (part - groups.first[e]) * each;
+    return Tile{e, rt * kGtRows, groups.starts[e] + skip, min(each, n - skip)};
   };
   const int steps = (a.K * (FP8 ? 1 : 2) + 127) >> 7;
   auto stage_w = [&](int s) { return base + s * kGtStage; };
@@ -529,6 +487,13 @@ static bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, in
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whether the few-rows kernel runs (vx_grouped_few.cu).  E = 512, K = 2,048,
+// N = 1,024, tiles / few rows: 1 token bf16 17.0 / 11.9 us, 64 247 / 226, 128
+// (2.5 rows an expert) 312 / 295, 256 (5) 344 / 336, but e4m3 192 / 196 and
+// 512 tokens (10) 195 / 279; E = 8, 4 rows an expert 17.7 / 9.8.  A handful
+// of positions is one item whatever the bank's size.
+static bool few_rows(int64_t P, int experts) { return P <= 4 * int64_t(experts) || P <= 8; }
+
 // Whether the rows are gathered by a launch of their own.  gather4 copies in
 // the product take its TMA unit 57 cycles per four rows.  E = 512, K = 2,048,
 // N = 1,024, gathered in the product / first: 5 rows an expert bf16 344 / 346
@@ -555,6 +520,7 @@ static cudaError_t launch_grouped_as(const GroupedTc& g, int pairs, cudaStream_t
 
 cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st) {
   if (a.P == 0 || a.N == 0) return cudaSuccess;
+  if (few_rows(a.P, a.experts)) return launch_grouped_few(a, e4m3, st);
   const int size = e4m3 ? 1 : 2;
   GroupedTc g;
   g.row_tiles = (a.N + kGtRows - 1) / kGtRows;

@@ -1,0 +1,84 @@
+// What the grouped products share: a position's row, and the table of groups
+// that each CTA builds in its shared memory.
+#pragma once
+
+#include "vx_common.cuh"
+#include "vx_launch.h"
+
+namespace vx {
+
+// The row of x that position p reads; -1 where it lies outside x.
+VX_DEVICE int row_of(const GroupedArgs& a, int p) {
+  const int r = __ldg(a.rows + p);
+  return r >= 0 && r / a.slots < a.x_rows ? r / a.slots : -1;
+}
+
+// Starts of the groups, clamped to [0, P] (group e is starts[e] ..
+// starts[e + 1], empty if that descends), and the exclusive scan of the
+// number of items that each is cut into (at most `most` positions an item).
+// Every thread of the CTA constructs it; memory: 2 (experts + 1) ints.
+template <int THREADS>
+struct GroupTable {
+  int* first;    // items before expert e
+  int* starts;
+  int experts, most;
+
+  VX_DEVICE GroupTable(const GroupedArgs& a, int* memory, int most_) : experts(a.experts), most(most_) {
+    __shared__ int scan[THREADS / 32];
+    first = memory;
+    starts = memory + experts + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // a thread takes neighbouring experts, all its loads at once
+    const int P = int(a.P), each = (experts + THREADS - 1) / THREADS, e0 = threadIdx.x * each;
+    auto start = [&](int e) { return min(max(__ldg(a.offsets + e), 0), P); };
+    int v = 0;
+    for (int i = 0, lo = e0 < experts ? start(e0) : 0; i < each && e0 + i < experts; ++i) {
+      const int hi = start(e0 + i + 1);
+      starts[e0 + i] = lo;
+      first[e0 + i] = v;   // inside the thread's range
+      v += (max(hi - lo, 0) + most - 1) / most;
+      if (e0 + i + 1 == experts) starts[experts] = hi;
+      lo = hi;
+    }
+    int up = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xFFFFFFFFu, up, o);
+      if (lane >= o) up += u;
+    }
+    if (lane == 31) scan[warp] = up;
+    __syncthreads();
+    int before = up - v, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += scan[w];
+      all += scan[w];
+    }
+    for (int i = 0; i < each && e0 + i < experts; ++i) first[e0 + i] += before;
+    if (threadIdx.x == 0) first[experts] = all;
+    __syncthreads();
+  }
+
+  VX_DEVICE int items() const { return first[experts]; }
+
+  // The expert that item i belongs to.
+  VX_DEVICE int expert(int i) const {
+    int lo = 0, hi = experts;   // the last e with first[e] <= i
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (first[m] <= i) lo = m; else hi = m;
+    }
+    return lo;
+  }
+  VX_DEVICE int size(int e) const { return starts[e + 1] - starts[e]; }   // of a group with items
+
+  // Item i of full items and a rest: its expert, first position and number of positions.
+  VX_DEVICE int item(int i, int* e, int* p0) const {
+    *e = expert(i);
+    const int skip = (i - first[*e]) * most;
+    *p0 = starts[*e] + skip;
+    return min(most, size(*e) - skip);
+  }
+};
+
+}  // namespace vx

@@ -916,7 +916,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     ``w_scales`` float32 [E, N] (one scale per row of x and of w).  Returns
     bf16 [P, N], P the length of ``rows`` (or M); positions from
     ``offsets[E]`` on are left as they were in ``out`` (undefined when it is
-    allocated here).  K must be a multiple of 16 bytes."""
+    allocated here).  K must be a multiple of 16 bytes, E at most 2048.  The
+    same call gives the same bits; another number of rows may take another
+    kernel, whose float32 sums run in another order."""
     e4m3 = isinstance(x, torch.Tensor) and x.dtype is torch.float8_e4m3fn
     if not e4m3 and not (isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16):
         raise TypeError("x must be a bfloat16 or float8_e4m3fn tensor")
