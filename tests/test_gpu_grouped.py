@@ -180,6 +180,50 @@ def test_calls_repeat_and_rows_do_not_depend_on_their_neighbours(kind, counts):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("counts", [[140], [129, 300], [256, 257, 512, 1, 0, 700], [1100, 3]],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("N", [1, 127, 130, 257, 512, 636])
+def test_many_rows(kind, counts, N):
+    """More than 128 rows an expert and rows of more than 512 bytes: the CTA pairs' tiles,
+    sorted rows and gathered ones, odd and wider out, special values in another group."""
+    K, P = 528 if kind == "e4m3" else 264, sum(counts)
+    x, w, xs, ws = operands(kind, P, len(counts), N, K, seed=21)
+    offsets = offsets_of(counts)
+    clean = check(x, w, offsets, f"{kind} {counts} N={N}", x_scales=xs, w_scales=ws)
+    rows = torch.randint(0, 2 * P, (P,), device="cuda", generator=gen(22), dtype=torch.int32)
+    check(x, w, offsets, f"{kind} {counts} N={N} rows", rows=rows, slots=2, x_scales=xs, w_scales=ws)
+    out = torch.full((P, N + 9), 5.0, dtype=torch.bfloat16, device="cuda")
+    check(x, w, offsets, f"{kind} {counts} N={N} out", x_scales=xs, w_scales=ws, out=out[:, 3:3 + N])
+    assert bool((out[:, :3] == 5).all()) and bool((out[:, 3 + N:] == 5).all())
+    if len(counts) > 1:
+        x2, w2 = x.clone(), w.clone()
+        x2.view(torch.uint8)[:counts[0]] = 0xFF
+        w2.view(torch.uint8)[0] = 0xFF
+        got = vxmoe.grouped_matmul(x2, w2, offsets, x_scales=xs, w_scales=ws)
+        assert got[:counts[0]].float().isnan().all()
+        assert torch.equal(got[counts[0]:].view(torch.int16), clean[counts[0]:].view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("counts", [[9], [64, 65], [0, 63, 128, 129, 17, 0, 1], [30] * 9 + [110]],
+                         ids=lambda c: "-".join(map(str, c[:8])))
+@pytest.mark.parametrize("N", [1, 127, 130, 256, 272, 636])
+def test_tens_of_rows(kind, counts, N):
+    """Tiles of up to 64 and up to 128 positions."""
+    K, P = 272, sum(counts)
+    x, w, xs, ws = operands(kind, P, len(counts), N, K, seed=23)
+    offsets = offsets_of(counts)
+    clean = check(x, w, offsets, f"{kind} {counts} N={N}", x_scales=xs, w_scales=ws)
+    rows = torch.randint(0, 3 * P, (P,), device="cuda", generator=gen(24), dtype=torch.int32)
+    check(x, w, offsets, f"{kind} {counts} N={N} rows", rows=rows, slots=3, x_scales=xs, w_scales=ws)
+    for wide in (9, 16):
+        out = torch.full((P, N + wide + 16 - N % 16), 5.0, dtype=torch.bfloat16, device="cuda")
+        got = check(x, w, offsets, f"{kind} {counts} N={N} out", x_scales=xs, w_scales=ws, out=out[:, wide:wide + N])
+        assert bool((out[:, :wide] == 5).all()) and bool((out[:, wide + N:] == 5).all())
+        assert torch.equal(got.contiguous().view(torch.int16), clean.view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 @pytest.mark.parametrize("E,P", [(1, 1), (1, 8), (3, 12), (40, 37), (512, 10), (512, 700), (2048, 9)])
 @pytest.mark.parametrize("N,K", [(16, 64), (33, 176), (1000, 2048), (128, 4112)])
 def test_few_rows(kind, E, P, N, K):

@@ -6,35 +6,32 @@
 // rows[p] / slots, or p itself; the scales only with e4m3.  Sums in float32,
 // one rounding.  Positions from offsets[E] on are left as they were.
 //
-// Few rows an expert go to vx_grouped_few.cu.  Here, a CTA pair (cluster of
-// two, cta_group::2) computes tiles of 256 outputs x
+// Three kernels, by the rows that an expert has on average (launch_grouped):
+// few, vx_grouped_few.cu; tens, vx_grouped_mid.cu; here, more than a hundred.
+// With `rows`, the latter two have x gathered by a launch of its own first.
+//
+// A CTA pair (cluster of two, cta_group::2) computes tiles of 256 outputs x
 // up to 256 positions of one expert with tcgen05.mma:
 //
 //   D[256 outputs][N positions] += W[256][K] . X[N][K]^T
 //
 // The bank's rows are the MMA's M side, so a group of any size fills it and
-// only N follows the ragged group (a multiple of 32): a group of one position
-// costs the bank's bytes and little else.  Each CTA of the pair stages its
-// own 128 bank rows and half of the positions, 128 bytes of K at a time
-// (64 bf16 or 128 e4m3 inputs), so a 256 x 256 tile moves 32 KB per CTA and
-// step through L2 where two single CTAs would move 48.  K past the end and
-// rows past a bank's outputs arrive as zeros.
+// only N follows the ragged group (a multiple of 32).  Each CTA of the pair
+// stages its own 128 bank rows and half of the positions, 128 bytes of K at a
+// time (64 bf16 or 128 e4m3 inputs), so a 256 x 256 tile moves 32 KB per CTA
+// and step through L2 where two single CTAs would move 48.  K past the end
+// and rows past a bank's outputs arrive as zeros.  With one group of 16,384
+// rows, K = N = 4,096, it runs at 1.46 PFLOP/s, 0.91 of the library's product;
+// what holds it is the power limit (1.4 GHz in steady state).
 //
 // Warp roles of a CTA (384 threads):
-//   warp 0      TMA: the bank rows and, without `rows`, the positions (boxes
-//               of 128, 64, 32 and 16 rows that add up to them) into a ring
-//               of kGtStages stages.  Both CTAs' copies complete on the
-//               leader's barrier.
+//   warp 0      TMA: the bank rows and the positions (boxes of 128, 64, 32 and
+//               16 rows that add up to them) into a ring of kGtStages stages.
+//               Both CTAs' copies complete on the leader's barrier.
 //   warp 1      leader only: one thread issues the MMAs of both CTAs and
 //               commits each stage back to both producers.
-//   warps 2, 3  with `rows`: gather4 copies, four rows of x each.  One thread
-//               a warp issues them with its row numbers from shared memory:
-//               the copy takes its operands in uniform registers, and 32
-//               lanes that issue one each are served one after the other
-//               (about 75 cycles a copy, 2,400 for the 128 rows of a stage
-//               whose MMAs take 512).  Warp 2 also allocates TMEM: two
-//               accumulators of 256 columns, so that a tile's epilogue runs
-//               beside the next tile's MMAs.
+//   warp 2      allocates TMEM: two accumulators of 256 columns, so that a
+//               tile's epilogue runs beside the next tile's MMAs.
 //   warps 4-11  epilogue: TMEM lane = output, column = position.  Four lanes
 //               exchange 4 x 4 values so that a lane stores four neighbouring
 //               outputs of one position (8 bytes; single outputs where out's
@@ -47,8 +44,7 @@
 // ...  Tiles are numbered expert by expert (prefix sums over the groups in
 // shared memory), so pairs running side by side share one bank and its
 // positions in L2.  A group of more than 256 positions is cut into equal
-// tiles rather than full ones and a rest.  A batch with many rows a group has
-// them gathered by a kernel of its own first (gather_first).
+// tiles rather than full ones and a rest.
 //
 // Every wait is bounded: one that runs out ends the CTA's roles, and the
 // tiles left over are filled with NaN.
@@ -71,8 +67,8 @@ constexpr int kGtStage = 2 * kGtHalf;               // bank rows, positions
 constexpr int kGtEpiWarps = 8;
 
 struct GroupedTc {
-  CUtensorMap tm_w, tm_x[4];                        // x: boxes of 16, 32, 64 and 128 rows (with `rows`: of one)
-  GroupedArgs a;
+  CUtensorMap tm_w, tm_x[4];                        // x: boxes of 16, 32, 64 and 128 rows
+  GroupedArgs a;                                    // rows null
   int row_tiles;                                    // 256-output tiles of a bank
   int by_four;                                      // out's rows take 8-byte stores
 };
@@ -89,7 +85,8 @@ VX_DEVICE uint32_t in_cta(uint32_t addr, uint32_t rank) {
   return r;
 }
 VX_DEVICE void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  __syncwarp();   // whole warps arrive and wait
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 VX_DEVICE void arrive_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
@@ -109,13 +106,6 @@ VX_DEVICE void pair_load_2d(uint32_t dst, const void* map, int x, int y, uint32_
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
       "[%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-VX_DEVICE void pair_gather4(uint32_t dst, const void* map, int x, int4 r, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(bar)
       : "memory");
 }
 
@@ -150,33 +140,6 @@ VX_DEVICE uint32_t pair_idesc(int n) {
   return (1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(kGtRows >> 4) << 24);
 }
 
-// mbar_try that also acquires what the other CTA of the pair released.
-VX_DEVICE bool pair_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-VX_DEVICE uint32_t bf16_pair(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// Bounded wait of a role: false once this CTA has given up.
-VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (pair_try(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    if (pair_try(bar, parity)) return true;
-    if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
-  }
-  *dead = 1;
-  return false;
-}
-
 // A tile: expert, first output, first position and number of positions.  The
 // MMA's N columns are two halves, one staged by each CTA: the first holds
 // positions 0 .. split(), the second the others, both padded to half().
@@ -188,12 +151,11 @@ struct Tile {
   VX_DEVICE int count(int h) const { return h ? n - split() : split(); }  // real columns of half h
 };
 
-template <bool FP8, bool GATHER>
+template <bool FP8>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedTc g) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kGtStages], empty[kGtStages], acc_full[2], acc_empty[2];
-  __shared__ __align__(16) int4 row_of_4[2][kGtCols / 2 / 8];   // warps 2, 3: rows of each copy
   __shared__ __align__(16) float x_scale[FP8 ? kGtEpiWarps : 1][kGtCols / 2];   // an epilogue warp's columns
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
@@ -219,11 +181,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  if (warp == 1 && lane < 5) {
-    const void* m = lane == 4 ? &g.tm_w : &g.tm_x[lane];
-    if (lane == 4 || lane == 0 || !GATHER)
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-  }
+  if (warp == 1 && lane < 5) prefetch_map(lane == 4 ? &g.tm_w : &g.tm_x[lane]);
   chain_wait();
 
   const GroupTable<kGtThreads> groups(a, table, kGtCols);
@@ -254,14 +212,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     for (int t = pair; ok && t < tiles; t += pairs) {
       const Tile c = tile_at(t);
       const int p0 = c.first(rank), w0 = c.row0 + rank * 128;
-      // rows copied by each CTA: its real positions, rounded up to the copies' size
-      constexpr int kUnit = GATHER ? 4 : 16;
-      auto copied = [&](int r) { return (c.count(r) + kUnit - 1) & ~(kUnit - 1); };
+      // rows copied by each CTA: its real positions, rounded up to the smallest box
+      auto copied = [&](int r) { return (c.count(r) + 15) & ~15; };
       const int mine = copied(rank);
       const uint32_t bytes = 2 * kGtHalf + (copied(0) + copied(1)) * 128;
       // lane i < 4 copies the box of 16 << i rows if `mine` has that bit; the
       // larger boxes come first, so box i starts at the bits above it
-      const bool box = !GATHER && lane < 4 && ((mine >> (4 + lane)) & 1);
+      const bool box = lane < 4 && ((mine >> (4 + lane)) & 1);
       const int at = mine & ~((32 << lane) - 1);
       for (int k = 0; k < steps; ++k) {
         if (!role_wait(smem_u32(&empty[s]), ph, &dead)) {
@@ -313,45 +270,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         if (++b == 2) b = 0, aph ^= 1;
       }
     }
-  } else if (GATHER && (warp == 2 || warp == 3)) {
-    // ---- rows of x: this warp's copies are 0, 2, ... or 1, 3, ... of a stage
-    const int w = warp - 2;
-    int s = 0;
-    uint32_t ph = 1;
-    bool ok = true;
-    for (int t = pair; ok && t < tiles; t += pairs) {
-      const Tile c = tile_at(t);
-      const int p0 = c.first(rank), mine = c.count(rank);
-      const int copies = ((mine + 3) / 4 - w + 1) / 2;
-      __syncwarp();
-      if (lane < 16) {
-        int r[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int q = 4 * (2 * lane + w) + j;
-          r[j] = q < mine ? max(row_of(a, p0 + q), 0) : 0;   // those columns are zeroed or not stored
-        }
-        row_of_4[w][lane] = make_int4(r[0], r[1], r[2], r[3]);
-      }
-      __syncwarp();
-      if (lane == 0) {
-        for (int k = 0; k < steps; ++k) {
-          ok = role_wait(smem_u32(&empty[s]), ph, &dead);
-          if (!ok) break;
-          const uint32_t bar = in_cta(smem_u32(&full[s]), 0), dst = stage_x(s) + w * 512;
-#pragma unroll 4
-          for (int j = 0; j < copies; ++j)
-            pair_gather4(dst + j * 1024, &g.tm_x[0], k * (FP8 ? 128 : 64), row_of_4[w][j], bar);
-          if (++s == kGtStages) s = 0, ph ^= 1;
-        }
-      }
-      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-    }
   } else if (warp >= 4) {
     // ---- epilogue: warp = a quarter of the outputs, half h of the positions
     const int quarter = warp & 3, h = (warp - 4) >> 2;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    float* scale = x_scale[warp - 4];
+    float* scale = x_scale[FP8 ? warp - 4 : 0];
     const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
     int b = 0;
     uint32_t ph = 0;
@@ -362,16 +285,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
       const int n = c.row0 + int(rank) * 128 + quarter * 32 + lane;   // this lane's output
       float sw = 1.f;
       if (FP8 && n < a.N) sw = __ldg(a.w_scales + int64_t(c.e) * a.N + n);
-      uint32_t outside[kGtCols / 64] = {};   // columns whose row lies outside x: zero
-      if (FP8 || GATHER) {
+      if (FP8) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kGtCols / 64; ++i) {
           const int col = 32 * i + lane;
-          int row = 0;
-          if (col < cols) row = GATHER ? row_of(a, p0 + col) : p0 + col;
-          if (FP8) scale[col] = col < cols && row >= 0 ? __ldg(a.x_scales + row) : 0.f;
-          if (GATHER) outside[i] = __ballot_sync(0xFFFFFFFFu, row < 0);
+          scale[col] = col < cols ? __ldg(a.x_scales + p0 + col) : 0.f;
         }
         __syncwarp();
       }
@@ -394,11 +313,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
             const float4 f = *reinterpret_cast<const float4*>(scale + c0 + 4 * j);
             v[4 * j] *= f.x * sw, v[4 * j + 1] *= f.y * sw, v[4 * j + 2] *= f.z * sw, v[4 * j + 3] *= f.w * sw;
           }
-        }
-        if (GATHER && outside[i >> 1]) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if ((outside[i >> 1] >> (16 * (i & 1) + j)) & 1u) v[j] = 0.f;
         }
         if (!ok) {
 #pragma unroll
@@ -473,7 +387,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn_grouped() {
 }
 
 // 128 bytes of K (128-byte swizzle) x `box_rows` rows of [outer][rows][K].
-static bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t rows, int64_t ld, int64_t outer,
+bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t rows, int64_t ld, int64_t outer,
                           int box_rows) {
   auto fn = encode_fn_grouped();
   if (!fn) return false;
@@ -487,73 +401,81 @@ static bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, in
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Whether the few-rows kernel runs (vx_grouped_few.cu).  E = 512, K = 2,048,
-// N = 1,024, tiles / few rows: 1 token bf16 17.0 / 11.9 us, 64 247 / 226, 128
-// (2.5 rows an expert) 312 / 295, 256 (5) 344 / 336, but e4m3 192 / 196 and
-// 512 tokens (10) 195 / 279; E = 8, 4 rows an expert 17.7 / 9.8.  A handful
-// of positions is one item whatever the bank's size.
+// Which kernel runs, by the positions P of E experts.
+//
+// Few rows (vx_grouped_few.cu) against the tiles here, E = 512, K = 2,048, N =
+// 1,024: 1 token bf16 11.9 / 17.0 us, 64 226 / 247, 128 (2.5 rows an expert)
+// 295 / 312, 256 (5) 336 / 344 but e4m3 196 / 192, 512 (10) 279 / 195; E = 8
+// and 4 rows an expert 9.8 / 17.7.  A handful of positions is one item
+// whatever the bank's size.
 static bool few_rows(int64_t P, int experts) { return P <= 4 * int64_t(experts) || P <= 8; }
-
-// Whether the rows are gathered by a launch of their own.  gather4 copies in
-// the product take its TMA unit 57 cycles per four rows.  E = 512, K = 2,048,
-// N = 1,024, gathered in the product / first: 5 rows an expert bf16 344 / 346
-// us, 10 e4m3 207 / 200, 40 e4m3 226 / 215, 160 e4m3 401 / 297; 4 tokens 26 /
-// 28 us, so a few rows in all stay in the product too.
-static bool gather_first(int64_t P, int experts) { return P >= 1024 && P >= 8 * int64_t(experts); }
+// Tens of rows (vx_grouped_mid.cu) against the tiles here, the same bank: 10
+// rows an expert e4m3 178 / 195 us, 20 bf16 344 / 365, 40 e4m3 200 / 213, 80
+// e4m3 230 / 239, E = 64 and 128 rows 72 / 75; 160 e4m3 333 / 299, bf16 607 /
+// 539.  Banks of short rows (K = 512 e4m3: four steps a tile, which does not
+// cover the epilogue here) 160 rows 185 / 248, 40 98 / 172.
+static bool mid_rows(int64_t P, int experts, int64_t row_bytes) {
+  return P <= 128 * int64_t(experts) || row_bytes <= 512;
+}
 
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows) {
-  if (!rows || !gather_first(P, experts)) return 0;
+  if (!rows || few_rows(P, experts)) return 0;
   const int64_t row = int64_t(K) * (e4m3 ? 1 : 2);
   return ((P * row + 255) & ~int64_t(255)) + (e4m3 ? 4 * P : 0);
 }
 
-template <bool FP8, bool GATHER>
-static cudaError_t launch_grouped_as(const GroupedTc& g, int pairs, cudaStream_t st) {
-  auto k = grouped_kernel<FP8, GATHER>;
-  const int smem = kGtStages * kGtStage + 1024 + 2 * (g.a.experts + 1) * int(sizeof(int));
+// x and its scales in the order of the positions, in the workspace; a takes
+// their place.
+static cudaError_t gather_rows(GroupedArgs& a, bool e4m3, void* workspace, cudaStream_t st) {
+  const int size = e4m3 ? 1 : 2, row_bytes = a.K * size, chunks = row_bytes / 16, per = chunks < 256 ? 256 / chunks : 1;
+  unsigned char* rows = static_cast<unsigned char*>(workspace);
+  float* scales = e4m3 ? reinterpret_cast<float*>(rows + ((a.P * row_bytes + 255) & ~int64_t(255))) : nullptr;
+  int64_t ctas = (a.P + per - 1) / per;
+  if (ctas > 16 * int64_t(sm_count())) ctas = 16 * int64_t(sm_count());
+  const cudaError_t e = launch_chained(gather_rows_kernel, dim3(unsigned(ctas)), dim3(256), 0, st, a, row_bytes,
+                                       a.ldx * size, rows, scales);
+  a.x = rows;
+  a.x_rows = a.P;
+  a.ldx = a.K;
+  a.x_scales = scales;
+  a.rows = nullptr;
+  a.slots = 1;
+  return e;
+}
+
+template <bool FP8>
+static cudaError_t launch_pairs(const GroupedTc& g, int pairs, cudaStream_t st) {
+  auto k = grouped_kernel<FP8>;
+  constexpr int kRing = kGtStages * kGtStage + 1024;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k),
-                             kGtStages * kGtStage + 1024 + 2 * (kGroupedMaxExperts + 1) * int(sizeof(int)), done);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), kRing + 2 * (kGroupedMaxExperts + 1) * int(sizeof(int)),
+                             done);
   if (e != cudaSuccess) return e;
-  return launch_chained(k, dim3(2 * pairs), dim3(kGtThreads), size_t(smem), st, g);
+  return launch_chained(k, dim3(2 * pairs), dim3(kGtThreads),
+                        size_t(kRing + 2 * (g.a.experts + 1) * int(sizeof(int))), st, g);
 }
 
 cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st) {
   if (a.P == 0 || a.N == 0) return cudaSuccess;
   if (few_rows(a.P, a.experts)) return launch_grouped_few(a, e4m3, st);
-  const int size = e4m3 ? 1 : 2;
+  if (a.rows) {
+    const cudaError_t e = gather_rows(a, e4m3, workspace, st);
+    if (e != cudaSuccess) return e;
+  }
+  if (mid_rows(a.P, a.experts, int64_t(a.K) * (e4m3 ? 1 : 2))) return launch_grouped_mid(a, e4m3, st);
   GroupedTc g;
+  g.a = a;
   g.row_tiles = (a.N + kGtRows - 1) / kGtRows;
+  g.by_four = a.N % 4 == 0 && a.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 8 == 0;
   // no more pairs than the groups can have tiles
   const int64_t groups = (a.P + kGtCols - 1) / kGtCols + (a.P < a.experts ? a.P : a.experts);
   if (groups * g.row_tiles > 0x7FFFFFFF) return cudaErrorInvalidValue;
   int64_t pairs = sm_count() / 2;
   if (groups * g.row_tiles < pairs) pairs = groups * g.row_tiles;
-  if (a.rows && gather_first(a.P, a.experts)) {
-    const int row_bytes = a.K * size, chunks = row_bytes / 16, per = chunks < 256 ? 256 / chunks : 1;
-    unsigned char* rows = static_cast<unsigned char*>(workspace);
-    float* scales = e4m3 ? reinterpret_cast<float*>(rows + ((a.P * row_bytes + 255) & ~int64_t(255))) : nullptr;
-    int64_t ctas = (a.P + per - 1) / per;
-    if (ctas > 16 * int64_t(sm_count())) ctas = 16 * int64_t(sm_count());
-    const cudaError_t e = launch_chained(gather_rows_kernel, dim3(unsigned(ctas)), dim3(256), 0, st, a, row_bytes,
-                                         a.ldx * size, rows, scales);
-    if (e != cudaSuccess) return e;
-    a.x = rows;
-    a.x_rows = a.P;
-    a.ldx = a.K;
-    a.x_scales = scales;
-    a.rows = nullptr;
-    a.slots = 1;
-  }
-  g.a = a;
-  g.by_four = a.N % 4 == 0 && a.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 8 == 0;
   if (!encode_k_rows(&g.tm_w, a.w, e4m3, a.K, a.N, a.K, a.experts, 128)) return cudaErrorInvalidValue;
-  for (int i = 0; i < (a.rows ? 1 : 4); ++i)
-    if (!encode_k_rows(&g.tm_x[i], a.x, e4m3, a.K, a.x_rows, a.ldx, 0, a.rows ? 1 : 16 << i))
-      return cudaErrorInvalidValue;
-  const int n = int(pairs);
-  if (e4m3) return a.rows ? launch_grouped_as<true, true>(g, n, st) : launch_grouped_as<true, false>(g, n, st);
-  return a.rows ? launch_grouped_as<false, true>(g, n, st) : launch_grouped_as<false, false>(g, n, st);
+  for (int i = 0; i < 4; ++i)
+    if (!encode_k_rows(&g.tm_x[i], a.x, e4m3, a.K, a.x_rows, a.ldx, 0, 16 << i)) return cudaErrorInvalidValue;
+  return e4m3 ? launch_pairs<true>(g, int(pairs), st) : launch_pairs<false>(g, int(pairs), st);
 }
 
 }  // namespace vx

@@ -1,7 +1,8 @@
-// What the grouped products share: a position's row, and the table of groups
-// that each CTA builds in its shared memory.
+// What the grouped products share: a position's row, the table of groups that
+// each CTA builds in its shared memory, bounded waits, tensor maps.
 #pragma once
 
+#include "vx_async.cuh"
 #include "vx_common.cuh"
 #include "vx_launch.h"
 
@@ -11,6 +12,33 @@ namespace vx {
 VX_DEVICE int row_of(const GroupedArgs& a, int p) {
   const int r = __ldg(a.rows + p);
   return r >= 0 && r / a.slots < a.x_rows ? r / a.slots : -1;
+}
+
+// mbar_try that also acquires what the other CTA of the pair released.
+VX_DEVICE bool pair_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+VX_DEVICE uint32_t bf16_pair(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Bounded wait of a role: false once this CTA has given up.
+VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (pair_try(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    if (pair_try(bar, parity)) return true;
+    if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
+  }
+  *dead = 1;
+  return false;
 }
 
 // Starts of the groups, clamped to [0, P] (group e is starts[e] ..
@@ -80,5 +108,14 @@ struct GroupTable {
     return min(most, size(*e) - skip);
   }
 };
+
+VX_DEVICE void prefetch_map(const void* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
+// Tensor map of 128 bytes of K (128-byte swizzle) x `box_rows` rows of
+// [outer][rows][K] (outer 0: [rows][K]); false if it cannot be encoded.
+bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t rows, int64_t ld, int64_t outer,
+                   int box_rows);
 
 }  // namespace vx

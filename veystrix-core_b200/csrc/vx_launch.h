@@ -389,6 +389,8 @@ struct GroupedArgs {
 };
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows);   // 0: none
 cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st);
+// Tens of rows an expert, rows already gathered (vx_grouped_mid.cu).
+cudaError_t launch_grouped_mid(const GroupedArgs& a, bool e4m3, cudaStream_t st);
 // Few rows an expert (vx_grouped_few.cu).
 cudaError_t launch_grouped_few(const GroupedArgs& a, bool e4m3, cudaStream_t st);
 
