@@ -102,6 +102,31 @@ def test_positions_behind_the_last_group_are_left(kind, gather):
     assert bool((out == 3).all())
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("P,E,K", [(9, 4, 64), (300, 2, 528), (40, 1, 64)])
+def test_bad_offsets_touch_only_what_they_may(kind, P, E, K):
+    """Any offsets: nothing outside [0, P) is read or written, no position twice."""
+    x, w, xs, ws = operands(kind, P, E, 48, K)
+    g = torch.Generator().manual_seed(3)
+    for trial in range(12):
+        bad = torch.randint(-P, 2 * P, (E + 1,), generator=g).int()
+        if trial == 0:
+            bad = torch.tensor([0, P] * E + [0])[:E + 1].int()
+        if trial == 1:
+            bad[:] = -2**31
+            bad[-1] = 2**31 - 1
+        good = bad.clamp(0, P).cummax(0).values
+        guard = torch.full((P + 64, 48), 9.0, dtype=torch.bfloat16, device="cuda")
+        out = guard[32:32 + P]
+        vxmoe.grouped_matmul(x, w, bad.cuda(), x_scales=xs, w_scales=ws, out=out)
+        want = torch.full((P, 48), 9.0, dtype=torch.bfloat16, device="cuda")
+        vxmoe.grouped_matmul(x, w, good.cuda(), x_scales=xs, w_scales=ws, out=want)
+        assert torch.equal(out, want), f"{bad.tolist()}"
+        assert bool((guard[:32] == 9).all()) and bool((guard[32 + P:] == 9).all())
+        first, last = int(good[0]), int(good[-1])
+        assert bool((want[:first] == 9).all()) and bool((want[last:] == 9).all())
+
+
 def test_offsets_and_rows_out_of_range():
     """Offsets are clamped to [0, P] and to ascend; a row outside x gives zeros."""
     x, w, _, _ = operands("bf16", 20, 4, 24, 64)
@@ -109,7 +134,7 @@ def test_offsets_and_rows_out_of_range():
     bad = torch.tensor([-3, 6, 4, 1000, 30], dtype=torch.int32, device="cuda")
     vxmoe.grouped_matmul(x, w, bad, out=out)
     want, size = grouped64(x, w, torch.tensor([0, 6, 6, 20, 20]))
-    # expert 1 has the descending pair [6, 4): nothing; expert 2 goes on from 4
+    # expert 1 has the descending pair [6, 4): nothing; expert 2 goes on from 6
     again, size2 = grouped64(x[4:], w[2:3], torch.tensor([0, 16]))
     got = out.double()
     tol = sum_tol(64)

@@ -41,48 +41,64 @@ VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
   return false;
 }
 
-// Starts of the groups, clamped to [0, P] (group e is starts[e] ..
-// starts[e + 1], empty if that descends), and the exclusive scan of the
-// number of items that each is cut into (at most `most` positions an item).
-// Every thread of the CTA constructs it; memory: 2 (experts + 1) ints.
+// Starts of the groups, clamped to [0, P] and to ascend (group e is starts[e]
+// .. starts[e + 1], so all of them have P positions at most), and the
+// exclusive scan of the number of items that each is cut into (at most `most`
+// positions an item).  Every thread of the CTA constructs it; memory: 2
+// (experts + 1) ints.
 template <int THREADS>
 struct GroupTable {
   int* first;    // items before expert e
   int* starts;
   int experts, most;
 
-  VX_DEVICE GroupTable(const GroupedArgs& a, int* memory, int most_) : experts(a.experts), most(most_) {
-    __shared__ int scan[THREADS / 32];
-    first = memory;
-    starts = memory + experts + 1;
+  // Inclusive scan over the CTA's threads; *all: over all of them.
+  template <typename F>
+  VX_DEVICE static int scan(int v, F&& join, int* all) {
+    __shared__ int warps[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // a thread takes neighbouring experts, all its loads at once
-    const int P = int(a.P), each = (experts + THREADS - 1) / THREADS, e0 = threadIdx.x * each;
-    auto start = [&](int e) { return min(max(__ldg(a.offsets + e), 0), P); };
-    int v = 0;
-    for (int i = 0, lo = e0 < experts ? start(e0) : 0; i < each && e0 + i < experts; ++i) {
-      const int hi = start(e0 + i + 1);
-      starts[e0 + i] = lo;
-      first[e0 + i] = v;   // inside the thread's range
-      v += (max(hi - lo, 0) + most - 1) / most;
-      if (e0 + i + 1 == experts) starts[experts] = hi;
-      lo = hi;
-    }
-    int up = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xFFFFFFFFu, up, o);
-      if (lane >= o) up += u;
+      const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+      if (lane >= o) v = join(u, v);
     }
-    if (lane == 31) scan[warp] = up;
+    if (lane == 31) warps[warp] = v;
     __syncthreads();
-    int before = up - v, all = 0;
+    int before = 0, total = 0;   // 0: neutral for what is scanned here
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) before += scan[w];
-      all += scan[w];
+      if (w < warp) before = join(before, warps[w]);
+      total = join(total, warps[w]);
     }
-    for (int i = 0; i < each && e0 + i < experts; ++i) first[e0 + i] += before;
+    *all = total;
+    return join(before, v);
+  }
+
+  VX_DEVICE GroupTable(const GroupedArgs& a, int* memory, int most_) : experts(a.experts), most(most_) {
+    first = memory;
+    starts = memory + experts + 1;
+    // a thread takes neighbouring entries, all its loads at once
+    const int P = int(a.P), each = (experts + THREADS) / THREADS, e0 = threadIdx.x * each;
+    const int e1 = min(e0 + each, experts + 1);
+    int top = 0, all;
+    for (int e = e0; e < e1; ++e) {
+      top = max(top, min(__ldg(a.offsets + e), P));
+      starts[e] = top;   // among the thread's own
+    }
+    const int upper = scan(top, [](int x, int y) { return max(x, y); }, &all);   // of the threads up to this one
+    // what the threads before this one reach: entry e0 - 1 after their own pass
+    if (e0 < e1) first[e1 - 1] = upper;
+    __syncthreads();
+    const int before = e0 > 0 && e0 < e1 ? first[e0 - 1] : 0;
+    for (int e = e0; e < e1; ++e) starts[e] = max(starts[e], before);
+    __syncthreads();
+    int v = 0;
+    for (int e = e0; e < min(e1, experts); ++e) {
+      first[e] = v;   // inside the thread's range
+      v += (starts[e + 1] - starts[e] + most - 1) / most;
+    }
+    const int upto = scan(v, [](int x, int y) { return x + y; }, &all);
+    for (int e = e0; e < min(e1, experts); ++e) first[e] += upto - v;
     if (threadIdx.x == 0) first[experts] = all;
     __syncthreads();
   }

@@ -34,7 +34,8 @@ namespace vx {
 
 constexpr int kLoraThreads = 256;
 constexpr int kLoraWarps = kLoraThreads / 32;
-constexpr int kLoraSmall = kLoraThreads;
+constexpr int kLoraSmall = VX_LORA_SMALL;
+static_assert(kLoraSmall <= kLoraThreads, "a thread a token");
 
 VX_DEVICE uint32_t lora_cluster_rank() {
   uint32_t r;

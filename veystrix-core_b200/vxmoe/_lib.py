@@ -71,6 +71,8 @@ class VxMoEWeights(ctypes.Structure):
 
 PATH_AUTO, PATH_GEMV, PATH_GEMM = 0, 1, 2
 
+LORA_SMALL = 256   # tokens up to which vx_lora_add needs no workspace
+
 EP_MAX_RANKS = 8
 EP_IPC_HANDLE_BYTES = 64
 

@@ -772,6 +772,10 @@ def _row_view(t: torch.Tensor, name: str, dtype: torch.dtype, align: int = 1):
         raise RuntimeError(f"{name} must live on a CUDA device (no CPU path)")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {str(dtype)[6:]}, got {t.dtype}")
+    if t.dim() == 2 and t.is_contiguous():   # the ordinary case, with the fewest calls
+        d = t.shape[1]
+        if d and (align == 1 or not (t.data_ptr() % align or d * t.element_size() % align)):
+            return t, d
     if t.dim() != 2:
         if t.dim() < 1 or t.shape[-1] == 0:
             raise ValueError(f"{name} must have shape [..., width], got {tuple(t.shape)}")
@@ -916,8 +920,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     ``w_scales`` float32 [E, N] (one scale per row of x and of w).  Returns
     bf16 [P, N], P the length of ``rows`` (or M); positions from
     ``offsets[E]`` on are left as they were in ``out`` (undefined when it is
-    allocated here).  K must be a multiple of 16 bytes, E at most 2048.  The
-    same call gives the same bits; another number of rows may take another
+    allocated here), and ``out`` overlaps no input.  K must be a multiple of 16
+    bytes, E at most 2048.  The same call gives the same bits; another number of rows may take another
     kernel, whose float32 sums run in another order."""
     e4m3 = isinstance(x, torch.Tensor) and x.dtype is torch.float8_e4m3fn
     if not e4m3 and not (isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16):
@@ -953,8 +957,8 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
         P = rows.numel()
     elif slots != 1:
         raise ValueError("slots needs rows")
-    if slots < 1:
-        raise ValueError("slots must be at least 1")
+    if not 1 <= slots < 1 << 31:
+        raise ValueError(f"slots must be at least 1, got {slots}")
     if out is None:
         out = x.new_empty((P, N), dtype=torch.bfloat16)
     else:
@@ -986,8 +990,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     gets ``y + scales[e] * b[e] @ (a[e] @ x)``, a token whose adapter is
     outside [0, L) (-1: none) gets y.  a [L, R, K] and b [L, N, R] bf16;
     ``scales`` float32 [L]; ``ranks`` int32 [L]: only the first ranks[e] of
-    the R components count.  ``out`` may be y itself.  K and R are multiples
-    of 8, R at most 256."""
+    the R components count.  ``out`` may be y itself and
+    overlaps nothing else.  K and R are multiples of 8, R at most 256, L at
+    most 4096."""
     x2, ldx = _row_view(x, "x", torch.bfloat16, align=16)
     y2, ldy = _row_view(y, "y", torch.bfloat16)
     T, K = x2.shape
@@ -1024,7 +1029,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         if out.shape != y.shape or o2.data_ptr() != out.data_ptr():
             raise ValueError(f"out must be rows of shape {tuple(y.shape)}, got {tuple(out.shape)}")
     lib = _lib.load()
-    nbytes = lib.vx_lora_add_workspace(T, L, R)
+    nbytes = lib.vx_lora_add_workspace(T, L, R) if T > _lib.LORA_SMALL else 0
     # its own allocation: a captured graph keeps it in its own pool
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _call(dev, "lora_add", lib.vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
