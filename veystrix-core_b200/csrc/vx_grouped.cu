@@ -160,7 +160,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   const GroupedArgs& a = g.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = int(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   int* table = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)) + kGtStages * kGtStage);
@@ -189,7 +189,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   auto tile_at = [&](int t) {
@@ -243,32 +243,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         }
     }
   } else if (warp == 1 && rank == 0) {
-    // ---- MMAs of the pair
-    if (lane == 0) {
-      int s = 0, b = 0;
-      uint32_t ph = 0, aph = 1;
-      bool ok = true;
-      for (int t = pair; ok && t < tiles; t += pairs) {
-        const Tile c = tile_at(t);
-        const uint32_t idesc = pair_idesc<FP8>(2 * c.half()), d = tmem + b * kGtCols;
-        if (!role_wait(smem_u32(&acc_empty[b]), aph, &dead)) break;
+    // ---- MMAs of the pair: the whole warp waits, one lane issues
+    int s = 0, b = 0;
+    uint32_t ph = 0, aph = 1;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      const uint32_t idesc = uniform(pair_idesc<FP8>(2 * tile_at(t).half())), d = tmem + b * kGtCols;
+      ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&acc_empty[b]), aph, &dead));
+      tc_fence_after();
+      for (int k = 0; ok && k < steps; ++k) {
+        ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&full[s]), ph, &dead));
+        if (!ok) break;
         tc_fence_after();
-        for (int k = 0; k < steps; ++k) {
-          if (!role_wait(smem_u32(&full[s]), ph, &dead)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        if (elect_one()) {
           const uint64_t ad = sw128_desc(stage_w(s)), bd = sw128_desc(stage_x(s));
 #pragma unroll
           for (int i = 0; i < 4; ++i) pair_mma<FP8>(d, ad + 2 * i, bd + 2 * i, idesc, k > 0 || i > 0);
           pair_commit(smem_u32(&empty[s]));
-          if (++s == kGtStages) s = 0, ph ^= 1;
+          if (k + 1 == steps) pair_commit(smem_u32(&acc_full[b]));
         }
-        if (!ok) break;
-        pair_commit(smem_u32(&acc_full[b]));
-        if (++b == 2) b = 0, aph ^= 1;
+        __syncwarp();
+        if (++s == kGtStages) s = 0, ph ^= 1;
       }
+      if (++b == 2) b = 0, aph ^= 1;
     }
   } else if (warp >= 4) {
     // ---- epilogue: warp = a quarter of the outputs, half h of the positions

@@ -125,6 +125,19 @@ struct GroupTable {
   }
 };
 
+// True in one lane, the same one in every call, of a converged warp.  MMAs
+// issued under it in a loop that the whole warp runs keep their operands in
+// uniform registers; under `lane == 0` the compiler moves them there one by
+// one, and an MMA takes 120 cycles to issue however small it is (M = 256, N =
+// 32: 57 this way, N = 144: 72).
+VX_DEVICE bool elect_one() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
+}
+// v of lane 0, which the compiler then knows to be the same in all lanes.
+VX_DEVICE uint32_t uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+
 VX_DEVICE void prefetch_map(const void* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   const GroupedArgs& a = g.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = int(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   int* table = reinterpret_cast<int*>(smem_raw + (base - smem_u32(smem_raw)) + kMidStages * kMidStage);
 
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = uniform(tmem_slot);
 
   auto tile_at = [&](int t) {
     // an expert's tiles: full parts and a rest, each with all the row tiles
@@ -156,37 +156,35 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
         }
     }
   } else if (warp == 1) {
-    // ---- MMAs
-    if (lane == 0) {
-      int s = 0, b = 0;
-      uint32_t ph = 0, aph = 1;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const MidTile c = tile_at(t);
-        const int n = min(kMidOut, (a.N - c.n0 + 15) & ~15);
-        const uint32_t d = tmem + b * kMidOut;
-        // float32 accumulator, both operands K-major, M = 64 or 128; bf16 is format
-        // 1, e4m3 format 0 of kind::f8f6f4
-        const uint32_t f = FP8 ? 0u : 1u;
-        const uint32_t idesc = (1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(c.m() >> 4) << 24);
-        if (!role_wait(smem_u32(&acc_empty[b]), aph, &dead)) break;
+    // ---- MMAs: the whole warp waits, one lane issues
+    int s = 0, b = 0;
+    uint32_t ph = 0, aph = 1;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      const MidTile c = tile_at(t);
+      const int n = min(kMidOut, (a.N - c.n0 + 15) & ~15);
+      const uint32_t d = tmem + b * kMidOut;
+      // float32 accumulator, both operands K-major, M = 64 or 128; bf16 is
+      // format 1, e4m3 format 0 of kind::f8f6f4
+      const uint32_t f = FP8 ? 0u : 1u;
+      const uint32_t idesc = uniform((1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(c.m() >> 4) << 24));
+      ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&acc_empty[b]), aph, &dead));
+      tc_fence_after();
+      for (int k = 0; ok && k < steps; ++k) {
+        ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&full[s]), ph, &dead));
+        if (!ok) break;
         tc_fence_after();
-        for (int k = 0; k < steps; ++k) {
-          if (!role_wait(smem_u32(&full[s]), ph, &dead)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        if (elect_one()) {
           const uint64_t xd = sw128_desc(stage_x(s)), wd = sw128_desc(stage_w(s));
 #pragma unroll
           for (int i = 0; i < 4; ++i) mid_mma<FP8>(d, xd + 2 * i, wd + 2 * i, idesc, k > 0 || i > 0);
           mma_commit(smem_u32(&empty[s]));
-          if (++s == kMidStages) s = 0, ph ^= 1;
+          if (k + 1 == steps) mma_commit(smem_u32(&acc_full[b]));
         }
-        if (!ok) break;
-        mma_commit(smem_u32(&acc_full[b]));
-        if (++b == 2) b = 0, aph ^= 1;
+        __syncwarp();
+        if (++s == kMidStages) s = 0, ph ^= 1;
       }
+      if (++b == 2) b = 0, aph ^= 1;
     }
   } else if (warp >= 4) {
     // ---- epilogue: warp = a quarter of the positions, half h of the outputs
