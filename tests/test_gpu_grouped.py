@@ -230,11 +230,12 @@ def test_many_rows(kind, counts, N):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
-@pytest.mark.parametrize("counts", [[9], [64, 65], [0, 63, 128, 129, 17, 0, 1], [30] * 9 + [110]],
-                         ids=lambda c: "-".join(map(str, c[:8])))
+@pytest.mark.parametrize("counts", [[70], [64, 65], [0, 63, 128, 129, 17, 0, 1], [i * 37 % 97 for i in range(160)],
+                                    [(0, 64, 65, 1, 128, 129, 16, 15)[i % 8] for i in range(152)]],
+                         ids=lambda c: f"{len(c)}-" + "-".join(map(str, c[:8])))
 @pytest.mark.parametrize("N", [1, 127, 130, 256, 272, 636])
 def test_tens_of_rows(kind, counts, N):
-    """Tiles of up to 64 and up to 128 positions."""
+    """Tiles of up to 64 and up to 128 positions, with enough experts for them and without."""
     K, P = 272, sum(counts)
     x, w, xs, ws = operands(kind, P, len(counts), N, K, seed=23)
     offsets = offsets_of(counts)

@@ -6,9 +6,10 @@
 // rows[p] / slots, or p itself; the scales only with e4m3.  Sums in float32,
 // one rounding.  Positions from offsets[E] on are left as they were.
 //
-// Three kernels, by the rows that an expert has on average (launch_grouped):
-// few, vx_grouped_few.cu; tens, vx_grouped_mid.cu; here, more than a hundred.
-// With `rows`, the latter two have x gathered by a launch of its own first.
+// Three kernels, by the number of positions (few_rows, mid_rows): a few,
+// vx_grouped_few.cu; some tens an expert or short bank rows,
+// vx_grouped_mid.cu; else the tiles here.  With `rows`, the latter two have x
+// gathered by a launch of its own first.
 //
 // A CTA pair (cluster of two, cta_group::2) computes tiles of 256 outputs x
 // up to 256 positions of one expert with tcgen05.mma:
@@ -21,22 +22,23 @@
 // time (64 bf16 or 128 e4m3 inputs), so a 256 x 256 tile moves 32 KB per CTA
 // and step through L2 where two single CTAs would move 48.  K past the end
 // and rows past a bank's outputs arrive as zeros.  With one group of 16,384
-// rows, K = N = 4,096, it runs at 1.46 PFLOP/s, 0.91 of the library's product;
-// what holds it is the power limit (1.4 GHz in steady state).
+// rows, K = N = 4,096, it runs at 1.59 PFLOP/s, 0.98 of the library's product;
+// what holds it in steady state is the power limit.
 //
 // Warp roles of a CTA (384 threads):
 //   warp 0      TMA: the bank rows and the positions (boxes of 128, 64, 32 and
 //               16 rows that add up to them) into a ring of kGtStages stages.
 //               Both CTAs' copies complete on the leader's barrier.
-//   warp 1      leader only: one thread issues the MMAs of both CTAs and
-//               commits each stage back to both producers.
+//   warp 1      leader only: issues the MMAs of both CTAs and commits each
+//               stage back to both producers.
 //   warp 2      allocates TMEM: two accumulators of 256 columns, so that a
 //               tile's epilogue runs beside the next tile's MMAs.
 //   warps 4-11  epilogue: TMEM lane = output, column = position.  Four lanes
 //               exchange 4 x 4 values so that a lane stores four neighbouring
 //               outputs of one position (8 bytes; single outputs where out's
 //               rows do not allow it): 2-byte stores kept the warps at a tile
-//               for 13,800 cycles, of 16,000 to 33,000 that its MMAs take.
+//               for 13,800 cycles, of 16,000 that its MMAs take at K = 2,048.
+//               The next tile's place and scales are on their way meanwhile.
 // Only rows of real positions are copied; the columns of a tile's padding
 // hold what the ring held before and are not stored.  The real positions are
 // dealt evenly to the halves.
@@ -247,8 +249,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     int s = 0, b = 0;
     uint32_t ph = 0, aph = 1;
     bool ok = true;
+    int half = pair < tiles ? tile_at(pair).half() : 0;
     for (int t = pair; ok && t < tiles; t += pairs) {
-      const uint32_t idesc = uniform(pair_idesc<FP8>(2 * tile_at(t).half())), d = tmem + b * kGtCols;
+      const uint32_t idesc = uniform(pair_idesc<FP8>(2 * half)), d = tmem + b * kGtCols;
       ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&acc_empty[b]), aph, &dead));
       tc_fence_after();
       for (int k = 0; ok && k < steps; ++k) {
@@ -266,6 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         if (++s == kGtStages) s = 0, ph ^= 1;
       }
       if (++b == 2) b = 0, aph ^= 1;
+      if (t + pairs < tiles) half = tile_at(t + pairs).half();   // while the MMAs run
     }
   } else if (warp >= 4) {
     // ---- epilogue: warp = a quarter of the outputs, half h of the positions
@@ -276,21 +280,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     int b = 0;
     uint32_t ph = 0;
     bool ok = true;
+    // a tile and the scales that this lane brings for it, one tile ahead
+    struct Next {
+      Tile c;
+      float sw, sx[kGtCols / 64];
+    } next;
+    auto fetch = [&](int t) {
+      if (t >= tiles) return;
+      next.c = tile_at(t);
+      if (!FP8) return;
+      const int n = next.c.row0 + int(rank) * 128 + quarter * 32 + lane;
+      next.sw = n < a.N ? __ldg(a.w_scales + int64_t(next.c.e) * a.N + n) : 0.f;
+#pragma unroll
+      for (int i = 0; i < kGtCols / 64; ++i)
+        next.sx[i] = 32 * i + lane < next.c.count(h) ? __ldg(a.x_scales + next.c.first(h) + 32 * i + lane) : 0.f;
+    };
+    fetch(pair);
     for (int t = pair; t < tiles; t += pairs) {
-      const Tile c = tile_at(t);
+      const Tile c = next.c;
       const int cols = c.count(h), p0 = c.first(h);
       const int n = c.row0 + int(rank) * 128 + quarter * 32 + lane;   // this lane's output
-      float sw = 1.f;
-      if (FP8 && n < a.N) sw = __ldg(a.w_scales + int64_t(c.e) * a.N + n);
+      const float sw = next.sw;
       if (FP8) {
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < kGtCols / 64; ++i) {
-          const int col = 32 * i + lane;
-          scale[col] = col < cols ? __ldg(a.x_scales + p0 + col) : 0.f;
-        }
+        for (int i = 0; i < kGtCols / 64; ++i) scale[32 * i + lane] = next.sx[i];
         __syncwarp();
       }
+      fetch(t + pairs);
       if (ok) ok = role_wait(smem_u32(&acc_full[b]), ph, &dead);
       ok = __all_sync(0xFFFFFFFFu, ok);
       tc_fence_after();
@@ -398,25 +415,28 @@ bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t r
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Which kernel runs, by the positions P of E experts.
+// Which kernel runs, by the positions P of E experts (times in us, K = 2,048).
 //
-// Few rows (vx_grouped_few.cu) against the tiles here, E = 512, K = 2,048, N =
-// 1,024: 1 token bf16 11.9 / 17.0 us, 64 226 / 247, 128 (2.5 rows an expert)
-// 295 / 312, 256 (5) 336 / 344 but e4m3 196 / 192, 512 (10) 279 / 195; E = 8
-// and 4 rows an expert 9.8 / 17.7.  A handful of positions is one item
-// whatever the bank's size.
-static bool few_rows(int64_t P, int experts) { return P <= 4 * int64_t(experts) || P <= 8; }
-// Tens of rows (vx_grouped_mid.cu) against the tiles here, the same bank: 10
-// rows an expert e4m3 178 / 195 us, 20 bf16 344 / 365, 40 e4m3 200 / 213, 80
-// e4m3 230 / 239, E = 64 and 128 rows 72 / 75; 160 e4m3 333 / 299, bf16 607 /
-// 539.  Banks of short rows (K = 512 e4m3: four steps a tile, which does not
-// cover the epilogue here) 160 rows 185 / 248, 40 98 / 172.
-static bool mid_rows(int64_t P, int experts, int64_t row_bytes) {
-  return P <= 128 * int64_t(experts) || row_bytes <= 512;
+// Few rows (vx_grouped_few.cu) / the tiles here: N = 1,024, E = 512: one token
+// bf16 11.9 / 17.0, four 31 / 37, e4m3 22.6 / 24.8, 100 positions bf16 122 /
+// 121, e4m3 72 / 66; N = 2,048: E = 1 and 32 positions 7.8 / 11.7, 64 11.4 /
+// 12.1, 128 18.5 / 12.9, E = 8 and 64 15.4 / 18.5, 128 23 / 19.  In steady
+// state, under the power limit, 64 tokens over 512 bf16 experts 231 / 236 (the
+// memory-bound MMAs here cost more power), e4m3 cold 135 / 124.
+static bool few_rows(int64_t P, int experts, bool e4m3) { return P <= 64 || (!e4m3 && P <= 2 * int64_t(experts)); }
+// Tens of rows (vx_grouped_mid.cu) / the tiles here, E = 512, N = 1,024: 10
+// rows an expert e4m3 178 / 179, 40 bf16 368 / 377, 80 e4m3 230 / 227; E = 64,
+// 128 rows 72 / 71, 640 158 / 150.  Banks of short rows (K = 512, N = 2,048)
+// e4m3 40 rows 98 / 146, 160 183 / 198; bf16 160 270 / 267.  It cuts a bank
+// into half as many tiles, so they have to be enough for the SMs: E = 8, 16
+// rows 21.7 / 18.9.
+static bool mid_rows(const GroupedArgs& a, int64_t row_bytes) {
+  const int64_t groups = a.P < a.experts ? a.P : a.experts, tiles = groups * ((a.N + 255) / 256);
+  return (a.P <= 64 * int64_t(a.experts) || row_bytes <= 512) && tiles >= sm_count();
 }
 
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows) {
-  if (!rows || few_rows(P, experts)) return 0;
+  if (!rows || few_rows(P, experts, e4m3)) return 0;
   const int64_t row = int64_t(K) * (e4m3 ? 1 : 2);
   return ((P * row + 255) & ~int64_t(255)) + (e4m3 ? 4 * P : 0);
 }
@@ -454,12 +474,12 @@ static cudaError_t launch_pairs(const GroupedTc& g, int pairs, cudaStream_t st) 
 
 cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st) {
   if (a.P == 0 || a.N == 0) return cudaSuccess;
-  if (few_rows(a.P, a.experts)) return launch_grouped_few(a, e4m3, st);
+  if (few_rows(a.P, a.experts, e4m3)) return launch_grouped_few(a, e4m3, st);
   if (a.rows) {
     const cudaError_t e = gather_rows(a, e4m3, workspace, st);
     if (e != cudaSuccess) return e;
   }
-  if (mid_rows(a.P, a.experts, int64_t(a.K) * (e4m3 ? 1 : 2))) return launch_grouped_mid(a, e4m3, st);
+  if (mid_rows(a, int64_t(a.K) * (e4m3 ? 1 : 2))) return launch_grouped_mid(a, e4m3, st);
   GroupedTc g;
   g.a = a;
   g.row_tiles = (a.N + kGtRows - 1) / kGtRows;

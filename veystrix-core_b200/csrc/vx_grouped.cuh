@@ -105,14 +105,20 @@ struct GroupTable {
 
   VX_DEVICE int items() const { return first[experts]; }
 
-  // The expert that item i belongs to.
+  // The expert that item i belongs to: the last e with first[e] <= i.  Called
+  // by whole warps: 32 samples, then the entries between two of them (two
+  // reads of shared memory, where a binary search waits for nine).
   VX_DEVICE int expert(int i) const {
-    int lo = 0, hi = experts;   // the last e with first[e] <= i
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (first[m] <= i) lo = m; else hi = m;
-    }
-    return lo;
+    const int lane = threadIdx.x & 31, stride = (experts + 31) / 32;
+    auto last = [&](int from, int by, int end) {   // of from, from + by, ... below end
+      const int e = from + lane * by;
+      const uint32_t under = __ballot_sync(0xFFFFFFFFu, e < end && first[e] <= i);
+      return under ? from + (31 - __clz(under)) * by : -1;
+    };
+    int e = last(0, stride, experts);
+    const int end = min(e + stride, experts);
+    for (int from = e; from < end; from += 32) e = max(e, last(from, 1, end));
+    return e;
   }
   VX_DEVICE int size(int e) const { return starts[e + 1] - starts[e]; }   // of a group with items
 

@@ -5,22 +5,25 @@
 //
 //   D[128 positions][256 outputs] += X[128][K] . W[256][K]^T   (or 64 positions)
 //
-// The positions are the MMA's M side here and the bank its N side: an MMA
-// takes about 134 cycles whatever it multiplies up to 128 x 256, so this way
-// each passes 256 bank rows through one SM, where the tiles of vx_grouped.cu
-// pass 128; those are the better ones once the positions fill them (a CTA
-// pair shares its 256 positions there).  A tile of at most 64 positions takes
-// M = 64: the same time, less power, and with it higher clocks (2,048 tokens
-// over 512 e4m3 experts in steady state: 210 us at 1.48 GHz, 222 at 0.97 with
-// M = 128, 239 by the tiles of vx_grouped.cu).  The padding rows of X are not
+// The positions are the MMA's M side here and the bank its N side, so a tile
+// has 256 outputs on one SM (32 KB of the bank in flight a stage) where the
+// tiles of vx_grouped.cu have 128, TMEM holds a position's outputs side by
+// side, and a tile begins and ends without a word to another CTA: with short
+// bank rows (K = 512 e4m3: four stages a tile) that is what counts, 98 against
+// 146 us for 20,480 rows over 512 experts of 2,048 outputs.  From about a
+// hundred positions an expert on the pairs' tiles are better: they fill up to
+// 256 columns and share the bank's rows.  The padding rows of X are not
 // copied; they hold what the ring held before, and their rows of D are not
-// read.
+// read.  A tile of at most 64 positions takes M = 64: less power, and with it
+// higher clocks (2,048 tokens over 512 e4m3 experts in steady state 210 us,
+// 222 with M = 128 throughout).  Those 2,048 tokens: 199 us at full clocks for
+// 1.12 GB, 0.86 of the measured copy rate, the gathering of the rows included.
 //
 // Warp roles (384 threads, one CTA an SM, persistent):
 //   warp 0      TMA: 256 bank rows (32 KB) and the real positions' rows (boxes
 //               of 128, 64, 32 and 16) into a ring of kMidStages stages
-//   warp 1      allocates TMEM (two accumulators of 256 columns); one thread
-//               issues the MMAs
+//   warp 1      allocates TMEM (two accumulators of 256 columns) and issues
+//               the MMAs
 //   warps 4-11  epilogue: TMEM lane = position, column = output; a lane
 //               stores 16 neighbouring outputs at once (32 bytes) where out's
 //               rows allow it, else 4 or 1
