@@ -24,7 +24,7 @@ def test_add_rmsnorm_refusals(lib):
     def call(x=P16, ldx=64, res=P16, res_type=0, ldr=64, gain=P16, T=3, d=64, res_out=P16, y=P16, q=P16, scales=P16):
         return lib.vx_add_rmsnorm(x, ldx, res, res_type, ldr, gain, T, d, 1e-6, res_out, y, q, scales, None)
 
-    for kw in (dict(T=-1), dict(d=0), dict(T=1 << 31), dict(ldx=-1), dict(ldr=-1), dict(x=None), dict(gain=None),
+    for kw in (dict(T=-1), dict(d=0), dict(d=(1 << 29) + 8), dict(T=1 << 31), dict(ldx=-1), dict(ldr=-1), dict(x=None), dict(gain=None),
                dict(q=None), dict(scales=None), dict(y=None, q=None, scales=None), dict(res=None),
                dict(res_out=None)):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw
@@ -38,7 +38,7 @@ def test_swiglu_e4m3_refusals(lib):
     def call(g=P16, ldg=64, u=P16, ldu=64, rows=3, width=64, q=P16, scales=P16):
         return lib.vx_swiglu_e4m3(g, ldg, u, ldu, rows, width, q, scales, None)
 
-    for kw in (dict(rows=-1), dict(rows=1 << 31), dict(width=0), dict(ldg=-1), dict(ldu=-1), dict(g=None),
+    for kw in (dict(rows=-1), dict(rows=1 << 31), dict(width=0), dict(width=(1 << 29) + 8), dict(ldg=-1), dict(ldu=-1), dict(g=None),
                dict(u=None), dict(q=None), dict(scales=None)):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw
     assert call(rows=0, g=None) == _lib.VX_OK
@@ -53,7 +53,7 @@ def test_grouped_matmul_refusals(lib):
                                      space, nbytes, None)
 
     e4m3 = dict(dtype=2, xs=P16, ws=P16)
-    for kw in (dict(E=0), dict(E=2049), dict(N=0), dict(K=0), dict(K=4, ldx=8), dict(ldx=60), dict(ldx=68),
+    for kw in (dict(E=0), dict(E=2049), dict(N=0), dict(N=(1 << 29) + 1, ldo=1 << 30), dict(K=(1 << 29) + 8, ldx=1 << 30), dict(K=0), dict(K=4, ldx=8), dict(ldx=60), dict(ldx=68),
                dict(slots=0), dict(P=-1), dict(P=1 << 31), dict(x_rows=1 << 31, P=1), dict(x_rows=-1),
                dict(x_rows=7), dict(slots=2), dict(ldo=23), dict(xs=P16), dict(ws=P16), dict(dtype=2),
                dict(dtype=2, xs=P16), dict(K=56, ldx=64, **e4m3), dict(K=48, ldx=56, **e4m3), dict(x=None),
@@ -79,7 +79,8 @@ def test_lora_add_refusals(lib):
              nbytes=0):
         return lib.vx_lora_add(y, ldy, x, ldx, a, b, ids, None, None, L, T, K, N, R, out, ldo, ws, nbytes, None)
 
-    for kw in (dict(T=-1), dict(T=1 << 31), dict(L=0), dict(L=4097), dict(K=0), dict(K=60), dict(N=0), dict(R=0), dict(R=12),
+    for kw in (dict(T=-1), dict(T=1 << 31), dict(L=0), dict(L=4097), dict(K=0), dict(K=60), dict(K=(1 << 29) + 8, ldx=1 << 30), dict(N=0),
+               dict(N=512 * 65535 + 1, ldy=1 << 26, ldo=1 << 26), dict(R=0), dict(R=12),
                dict(R=264), dict(ldy=23), dict(ldo=23), dict(ldx=63), dict(ldx=68), dict(y=None), dict(x=None),
                dict(a=None), dict(b=None), dict(ids=None), dict(out=None), dict(x=ODD), dict(a=ODD), dict(b=ODD)):
         assert call(**kw) == _lib.VX_EINVAL_SHAPE, kw

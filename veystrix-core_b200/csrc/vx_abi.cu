@@ -59,6 +59,10 @@ struct Carver {
   size_t size() const { return (off + 255) & ~size_t(255); }
 };
 
+// Widths up to which the row, grouped and adapter kernels' 32-bit column
+// arithmetic holds.
+constexpr int kMaxWidth = 1 << 29;
+
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 static int check_q4(const vx_q4* b, int experts, int out, int in, int group = 32) {
@@ -1089,7 +1093,7 @@ int vx_rmsnorm(const uint16_t* x, const uint16_t* gain, int32_t T, int32_t d, fl
 int vx_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* residual, int32_t residual_dtype, int64_t ldr,
                    const uint16_t* gain, int64_t T, int32_t d, float eps, void* residual_out, uint16_t* y,
                    uint8_t* q, float* scales, void* stream) {
-  if (T < 0 || T > 0x7FFFFFFF || d < 1 || ldx < 0 || ldr < 0) return VX_EINVAL_SHAPE;
+  if (T < 0 || T > 0x7FFFFFFF || d < 1 || d > kMaxWidth || ldx < 0 || ldr < 0) return VX_EINVAL_SHAPE;
   if (residual && residual_dtype != VX_DTYPE_BF16 && residual_dtype != VX_DTYPE_F32) return VX_EINVAL_DTYPE;
   if (T == 0) return VX_OK;   // empty tensors may come as null pointers
   if ((q == nullptr) != (scales == nullptr) || (!y && !q) || (residual == nullptr) != (residual_out == nullptr))
@@ -1102,7 +1106,7 @@ int vx_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* residual, int32_t
 
 int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_t ldu, int64_t rows, int32_t width,
                    uint8_t* q, float* scales, void* stream) {
-  if (rows < 0 || rows > 0x7FFFFFFF || width < 1 || ldg < 0 || ldu < 0) return VX_EINVAL_SHAPE;
+  if (rows < 0 || rows > 0x7FFFFFFF || width < 1 || width > kMaxWidth || ldg < 0 || ldu < 0) return VX_EINVAL_SHAPE;
   if (rows == 0) return VX_OK;
   if (!gate || !up || !q || !scales) return VX_EINVAL_SHAPE;
   cudaError_t e = launch_swiglu_e4m3(gate, ldg, up, ldu, rows, width, q, scales, static_cast<cudaStream_t>(stream));
@@ -1121,7 +1125,9 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
                       int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return VX_EINVAL_DTYPE;
   const int size = dtype == VX_DTYPE_BF16 ? 2 : 1;
-  if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1) return VX_EINVAL_SHAPE;
+  if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1 || N > kMaxWidth ||
+      K > kMaxWidth)
+    return VX_EINVAL_SHAPE;
   // position numbers, with a tile's padding, stay within 32 bits
   if (P < 0 || P > 0x7FFF0000 || x_rows < 0 || x_rows > 0x7FFF0000 || ldo < N) return VX_EINVAL_SHAPE;
   if (!rows && (x_rows < P || slots != 1)) return VX_EINVAL_SHAPE;
@@ -1146,7 +1152,8 @@ int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, 
                 const int32_t* adapters, const float* scales, const int32_t* ranks, int32_t L, int64_t T, int32_t K,
                 int32_t N, int32_t R, uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                 void* stream) {
-  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || K < 8 || K % 8 || N < 1 || R < 8 || R % 8 || R > kLoraMaxRank)
+  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || K < 8 || K % 8 || K > kMaxWidth || N < 1 ||
+      N > kLoraMaxOut || R < 8 || R % 8 || R > kLoraMaxRank)
     return VX_EINVAL_SHAPE;
   if (ldy < N || ldo < N || ldx < K || ldx % 8) return VX_EINVAL_SHAPE;
   if (T == 0) return VX_OK;

@@ -397,6 +397,7 @@ cudaError_t launch_grouped_few(const GroupedArgs& a, bool e4m3, cudaStream_t st)
 // Low-rank adapters (vx_lora.cu).
 constexpr int kLoraMaxRank = 256;
 constexpr int kLoraMaxAdapters = 4096;
+constexpr int kLoraMaxOut = 512 * 65535;   // the expanding launch's grid
 struct LoraArgs {
   const uint16_t* y;            // [T][ldy]
   int64_t ldy;

@@ -126,9 +126,9 @@ VX_DEVICE int lora_rank(const LoraArgs& a, int e) {
 
 // A_e x of the item's n tokens over the 32-input blocks first, first + stride,
 // ... of the CTA's warps, 8 * NT components at a time; out(row, r, v) gets
-// four neighbouring sums of the CTA.  part: lora_part_floats.  AHEAD: the
-// next block's operands are loaded before the present one's MMAs.  ready() is
-// called by every thread once, before the first out().
+// four neighbouring sums of the CTA.  part: the warps' sums, 128 MT NT floats
+// each.  AHEAD: the next block's operands are loaded before the present one's
+// MMAs.  ready() is called by every thread once, before the first out().
 template <int MT, int NT, bool AHEAD, typename G, typename F>
 VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, int n, int first, int stride,
                            float* part, G&& ready, F&& out) {
@@ -302,23 +302,13 @@ VX_DEVICE void lora_expand(const LoraArgs& a, const uint16_t* B, int rank, const
     store8<WIDE>(a.out + t[i] * a.ldo, n, a.N, v);
   }
 }
-// The 32-output blocks first, first + stride, ... below `end`; the first
-// block's y and B are loaded by the caller.  AHEAD: each block's are loaded
-// before its predecessor is computed.
-template <int MT, int KB, bool WIDE, bool AHEAD>
+// The 32-output blocks first, first + stride, ... below `end`, each one's y
+// and B loaded before its predecessor is computed; the first block's are
+// loaded by the caller.
+template <int MT, int KB, bool WIDE>
 VX_DEVICE void lora_expand_all(const LoraArgs& a, const uint16_t* B, int rank, const uint4* frag,
                                const int (&t)[2 * MT], int first, int stride, int end, Eight<WIDE> (&y)[2 * MT],
                                uint4 (&bf)[KB][4]) {
-  if constexpr (!AHEAD) {
-    for (int nb = first; nb * 32 < end; nb += stride) {
-      if (nb != first) {
-        load_b<KB>(a, B, rank, nb, 0, bf);
-        load_y<MT, WIDE>(a, t, nb, y);
-      }
-      lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, y, bf);
-    }
-    return;
-  }
   Eight<WIDE> yn[2 * MT];
   uint4 bn[KB][4];
   int nb = first;
@@ -437,13 +427,12 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
     }
     __syncthreads();
   }
-  lora_expand_all<1, kSmallKb, WIDE, true>(a, B, rank, frag, t, nb0, stride, a.N, y, bf);
+  lora_expand_all<1, kSmallKb, WIDE>(a, B, rank, frag, t, nb0, stride, a.N, y, bf);
 }
 
 // ---- large batches ------------------------------------------------------------
 
 constexpr int kLargeMt = 2, kLargeTm = 16 * kLargeMt;
-
 constexpr int kLargeNt = 4, kLargeKb = 1;
 constexpr int kLargePart = kLoraWarps * kLargeTm * 8 * kLargeNt;   // floats
 
@@ -520,7 +509,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
     p[2] = v.y;   // 2, 3: two registers on
   }
   __syncthreads();
-  lora_expand_all<kLargeMt, kLargeKb, WIDE, true>(a, B, rank, frag, t, nb0, kLoraWarps, end, y, bf);
+  lora_expand_all<kLargeMt, kLargeKb, WIDE>(a, B, rank, frag, t, nb0, kLoraWarps, end, y, bf);
 }
 
 // One CTA: tokens counted per adapter (bucket L: none), buckets cut into
@@ -714,7 +703,6 @@ cudaError_t launch_lora(const LoraArgs& a, void* workspace, cudaStream_t st) {
   auto aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
   const bool wide = a.N % 8 == 0 && aligned(a.y, a.T > 1 ? a.ldy : 0) && aligned(a.out, a.T > 1 ? a.ldo : 0);
   if (a.T <= kLoraSmall) return wide ? launch_lora_small<true>(a, st) : launch_lora_small<false>(a, st);
-  if (a.N > 512 * 65535) return cudaErrorInvalidValue;
   char* ws = static_cast<char*>(workspace);
   return wide ? launch_lora_large<true>(a, ws, st) : launch_lora_large<false>(a, ws, st);
 }

@@ -814,16 +814,10 @@ def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
     return _i32(t, dev, name)
 
 
-def _call(dev: torch.device, what: str, fn, *args) -> None:
-    """fn(*args, stream) on dev's current stream, with dev current."""
-    index = dev.index
-    if torch.cuda.current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _lib.check(status, what)
+# What a call needs each time, without the Python layers of torch.cuda: the
+# small operators below are host-bound.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class AddNorm(NamedTuple):
@@ -848,6 +842,9 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
     x2, ldx = _row_view(x, "x", torch.bfloat16)
     T, d = x2.shape
     dev = x2.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return add_rms_norm(x, residual, gain, eps, output)
     gain = _bf16(gain, "gain")
     if gain.numel() != d:
         raise ValueError("gain must have the hidden size")
@@ -875,8 +872,10 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
     if output != "bf16":
         q = torch.empty_like(like, dtype=torch.float8_e4m3fn)
         scales = x2.new_empty(shape[:-1], dtype=torch.float32)
-    _call(dev, "add_rms_norm", _lib.load().vx_add_rmsnorm, x2.data_ptr(), ldx, _ptr(r2), res_type, ldr,
-          gain.data_ptr(), T, d, float(eps), _ptr(res_out), _ptr(y), _ptr(q), _ptr(scales))
+    status = _lib.load().vx_add_rmsnorm(x2.data_ptr(), ldx, _ptr(r2), res_type, ldr, gain.data_ptr(), T, d, float(eps),
+                                        _ptr(res_out), _ptr(y), _ptr(q), _ptr(scales), _raw_stream(dev.index))
+    if status:
+        _lib.check(status, "add_rms_norm")
     return AddNorm(y, res_out, q, scales)
 
 
@@ -897,12 +896,17 @@ def swiglu_e4m3(gate: torch.Tensor, up: torch.Tensor) -> E4M3Rows:
     dev = g2.device
     if u2.device != dev:
         raise _other_device("up", u2, dev)
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return swiglu_e4m3(gate, up)
     rows, width = g2.shape
     q = (torch.empty_like(gate, dtype=torch.float8_e4m3fn) if gate.is_contiguous()
          else gate.new_empty(gate.shape, dtype=torch.float8_e4m3fn))
     scales = g2.new_empty(gate.shape[:-1], dtype=torch.float32)
-    _call(dev, "swiglu_e4m3", _lib.load().vx_swiglu_e4m3, g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width,
-          q.data_ptr(), scales.data_ptr())
+    status = _lib.load().vx_swiglu_e4m3(g2.data_ptr(), ldg, u2.data_ptr(), ldu, rows, width, q.data_ptr(),
+                                        scales.data_ptr(), _raw_stream(dev.index))
+    if status:
+        _lib.check(status, "swiglu_e4m3")
     return E4M3Rows(q, scales)
 
 
@@ -928,9 +932,12 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
         raise TypeError("x must be a bfloat16 or float8_e4m3fn tensor")
     if x.dim() != 2:
         raise ValueError(f"x must have shape [rows, K], got {tuple(x.shape)}")
+    dev = x.device
+    if x.is_cuda and _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return grouped_matmul(x, w, offsets, rows, slots, x_scales, w_scales, out)
     x, ldx = _row_view(x, "x", x.dtype, align=16)
     M, K = x.shape
-    dev = x.device
     _require_cuda(w, "w")
     if w.dtype != x.dtype:
         raise TypeError(f"w must be {str(x.dtype)[6:]} as x, got {w.dtype}")
@@ -974,9 +981,11 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     nbytes = lib.vx_grouped_matmul_workspace(kind, P, E, K, 1) if rows is not None else 0
     # its own allocation: a captured graph keeps it in its own pool
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, "grouped_matmul", lib.vx_grouped_matmul, x.data_ptr(), kind, M, ldx, w.data_ptr(), _ptr(x_scales), _ptr(w_scales),
-          offsets.data_ptr(), E, N, K, _ptr(rows), int(slots), P, out.data_ptr(),
-          out.stride(0) if P > 1 else N, _ptr(ws), nbytes)
+    status = lib.vx_grouped_matmul(x.data_ptr(), kind, M, ldx, w.data_ptr(), _ptr(x_scales), _ptr(w_scales),
+                                   offsets.data_ptr(), E, N, K, _ptr(rows), int(slots), P, out.data_ptr(),
+                                   out.stride(0) if P > 1 else N, _ptr(ws), nbytes, _raw_stream(dev.index))
+    if status:
+        _lib.check(status, "grouped_matmul")
     return out
 
 
@@ -998,6 +1007,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     T, K = x2.shape
     N = y2.shape[1]
     dev = x2.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return lora_add(y, x, a, b, adapters, scales, ranks, out)
     _require_cuda(a, "a")
     _require_cuda(b, "b")
     if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
@@ -1032,7 +1044,9 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     nbytes = lib.vx_lora_add_workspace(T, L, R) if T > _lib.LORA_SMALL else 0
     # its own allocation: a captured graph keeps it in its own pool
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, "lora_add", lib.vx_lora_add, y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(),
-          b.data_ptr(), adapters.data_ptr(), _ptr(scales), _ptr(ranks), L, T, K, N, R, out.data_ptr(), ldo, _ptr(ws),
-          nbytes)
+    status = lib.vx_lora_add(y2.data_ptr(), ldy, x2.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), adapters.data_ptr(),
+                             _ptr(scales), _ptr(ranks), L, T, K, N, R, out.data_ptr(), ldo, _ptr(ws), nbytes,
+                             _raw_stream(dev.index))
+    if status:
+        _lib.check(status, "lora_add")
     return out
