@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(kGroupThreads) lora_group_kernel(const LoraArg
   __syncthreads();
   int2 next = make_int2(inc.x - own.x, inc.y - own.y);
   int total = 0;
-  for (int w = 0; w < 32; ++w) {
+  const int used = (buckets + 32 * per - 1) / (32 * per);   // warps that hold buckets
+  for (int w = 0; w < used; ++w) {
     if (w < warp) next.x += s_warp[w].x, next.y += s_warp[w].y;
     total += s_warp[w].y;
   }
