@@ -368,23 +368,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
 
 // ---- rows gathered first ------------------------------------------------------
 
-// x row of every position (zeros where it lies outside x), and its scale.
-__global__ void __launch_bounds__(256) gather_rows_kernel(const GroupedArgs a, int row_bytes, int64_t ld_bytes,
-                                                          unsigned char* __restrict__ rows_out,
-                                                          float* __restrict__ scales_out) {
+// x row of every position (zeros where it lies outside x), and its scale.  A
+// warp copies kGatherPiece bytes of a row, all of its loads at once: many
+// short warps hide the row number's latency better than fewer with several
+// rows each.  20,480 rows of 2,048 bytes take 10 us.
+constexpr int kGatherThreads = 256, kGatherAhead = 4, kGatherPiece = kGatherAhead * 512;
+
+__global__ void __launch_bounds__(kGatherThreads) gather_rows_kernel(const GroupedArgs a, int row_bytes,
+                                                                     int64_t ld_bytes,
+                                                                     unsigned char* __restrict__ rows_out,
+                                                                     float* __restrict__ scales_out) {
   chain_begin();
-  const int chunks = row_bytes / 16, per = blockDim.x / chunks > 0 ? blockDim.x / chunks : 1;
-  // a CTA takes `per` positions at a time (rows of at most 256 chunks side by side)
-  const int sub = threadIdx.x / chunks, c0 = per > 1 ? threadIdx.x - sub * chunks : threadIdx.x;
-  if (per > 1 && sub >= per) return;
-  for (int64_t p = int64_t(blockIdx.x) * per + (per > 1 ? sub : 0); p < a.P; p += int64_t(gridDim.x) * per) {
-    const int row = row_of(a, int(p));
-    const unsigned char* src = static_cast<const unsigned char*>(a.x) + (row < 0 ? 0 : row * ld_bytes);
-    for (int c = c0; c < chunks; c += per > 1 ? chunks : int(blockDim.x))
-      *reinterpret_cast<uint4*>(rows_out + p * row_bytes + c * 16) =
-          row < 0 ? make_uint4(0, 0, 0, 0) : ldg_nc(src + c * 16);
-    if (scales_out && c0 == 0) scales_out[p] = row < 0 ? 0.f : __ldg(a.x_scales + row);
-  }
+  const int lane = threadIdx.x & 31, pieces = (row_bytes + kGatherPiece - 1) / kGatherPiece;
+  const int64_t unit = int64_t(blockIdx.x) * (kGatherThreads / 32) + (threadIdx.x >> 5), p = unit / pieces;
+  if (p >= a.P) return;
+  const int from = int(unit - p * pieces) * kGatherPiece + lane * 16, row = row_of(a, int(p));
+  if (scales_out && from == 0) scales_out[p] = row < 0 ? 0.f : __ldg(a.x_scales + row);
+  const unsigned char* src = static_cast<const unsigned char*>(a.x) + (row < 0 ? 0 : row * ld_bytes);
+  unsigned char* dst = rows_out + p * row_bytes;
+  uint4 v[kGatherAhead];
+#pragma unroll
+  for (int u = 0; u < kGatherAhead; ++u)
+    v[u] = from + 512 * u < row_bytes && row >= 0 ? ldg_nc(src + from + 512 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int u = 0; u < kGatherAhead; ++u)
+    if (from + 512 * u < row_bytes) *reinterpret_cast<uint4*>(dst + from + 512 * u) = v[u];
 }
 
 // ---- host side --------------------------------------------------------------
@@ -444,13 +452,14 @@ int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool r
 // x and its scales in the order of the positions, in the workspace; a takes
 // their place.
 static cudaError_t gather_rows(GroupedArgs& a, bool e4m3, void* workspace, cudaStream_t st) {
-  const int size = e4m3 ? 1 : 2, row_bytes = a.K * size, chunks = row_bytes / 16, per = chunks < 256 ? 256 / chunks : 1;
+  const int size = e4m3 ? 1 : 2, row_bytes = a.K * size;
   unsigned char* rows = static_cast<unsigned char*>(workspace);
   float* scales = e4m3 ? reinterpret_cast<float*>(rows + ((a.P * row_bytes + 255) & ~int64_t(255))) : nullptr;
-  int64_t ctas = (a.P + per - 1) / per;
-  if (ctas > 16 * int64_t(sm_count())) ctas = 16 * int64_t(sm_count());
-  const cudaError_t e = launch_chained(gather_rows_kernel, dim3(unsigned(ctas)), dim3(256), 0, st, a, row_bytes,
-                                       a.ldx * size, rows, scales);
+  const int64_t units = a.P * ((row_bytes + kGatherPiece - 1) / kGatherPiece);
+  const int64_t ctas = (units + kGatherThreads / 32 - 1) / (kGatherThreads / 32);
+  if (ctas > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  const cudaError_t e = launch_chained(gather_rows_kernel, dim3(unsigned(ctas)), dim3(kGatherThreads), 0, st, a,
+                                       row_bytes, a.ldx * size, rows, scales);
   a.x = rows;
   a.x_rows = a.P;
   a.ldx = a.K;
