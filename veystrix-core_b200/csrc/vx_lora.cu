@@ -25,7 +25,7 @@
 //
 // Above: lora_group_kernel sorts the batch into items of 32 tokens,
 // lora_shrink_kernel (a CTA an item) writes h as bf16 pairs, and
-// lora_expand_kernel (a CTA an item and 512 or 1,024 outputs) streams y.
+// lora_expand_kernel (a CTA an item and 512 to 4,096 outputs) streams y.
 #include "vx_async.cuh"
 #include "vx_common.cuh"
 #include "vx_launch.h"
@@ -681,10 +681,17 @@ static cudaError_t launch_lora_large(const LoraArgs& a, char* ws, cudaStream_t s
   int4* items = reinterpret_cast<int4*>(ws + sp.items);
   uint16_t* h = reinterpret_cast<uint16_t*>(ws + sp.h);
   const unsigned n = unsigned(lora_max_items(a.T, a.L, kLargeTm));
-  // outputs of an expanding CTA: 1,024 spread its start over more blocks (8,192
-  // tokens x 4,096 outputs 54 against 56 us) while that leaves a CTA for every
-  // SM; else 512 (512 tokens: 22 against 24 us)
-  const int cols = int64_t(n) * ((a.N + 1023) / 1024) >= 2 * sm_count() ? 1024 : 512;
+  // Outputs of an expanding CTA: the number that costs least, a round of the
+  // resident CTAs taken as its outputs and 160 for its start, as long as three
+  // CTAs to two SMs are left.  8,192 tokens x 4,096 outputs take 52.2 us with
+  // 4,096, 54.1 with 1,024; 5,000 x 8,192 take 62.5 with 1,024, 64.2 with 512
+  // and with 2,048; 512 x 4,096 take 20.8 with 512, 23.1 with 1,024.
+  const int64_t resident = 2 * int64_t(sm_count());
+  int cols = 512;
+  for (int64_t c = 512, best = 0; c <= 4096; c *= 2) {
+    const int64_t ctas = int64_t(n) * ((a.N + c - 1) / c), cost = (ctas + resident - 1) / resident * (c + 160);
+    if (c == 512 || (4 * ctas >= 3 * resident && cost < best)) best = cost, cols = int(c);
+  }
   static std::atomic<uint64_t> done{0};
   auto expand = lora_expand_kernel<WIDE>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(expand), lora_frag_bytes(kLargeMt, kLoraMaxRank), done);
