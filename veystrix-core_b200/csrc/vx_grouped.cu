@@ -426,15 +426,16 @@ bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t r
 // Which kernel runs, by the positions P of E experts (times in us, K = 2,048).
 //
 // Few rows (vx_grouped_few.cu) / the tiles here: N = 1,024, E = 512: one token
-// bf16 11.9 / 17.0, four 31 / 37, e4m3 22.6 / 24.8, 100 positions bf16 122 /
-// 121, e4m3 72 / 66; N = 2,048: E = 1 and 32 positions 7.8 / 11.7, 64 11.4 /
-// 12.1, 128 18.5 / 12.9, E = 8 and 64 15.4 / 18.5, 128 23 / 19.  In steady
-// state, under the power limit, 64 tokens over 512 bf16 experts 231 / 236 (the
-// memory-bound MMAs here cost more power), e4m3 cold 135 / 124.
+// bf16 11.8 / 14.0, four 31 / 40, e4m3 19.6 / 24.8, 100 positions bf16 121 /
+// 121, e4m3 75 / 66; N = 2,048: E = 1 and 32 positions 8.1 / 12.4, 64 11.7 /
+// 12.8, 128 19 / 14, E = 8 and 64 15.8 / 18.6, 128 23 / 19.  64 tokens over 512
+// bf16 experts cold 234 / 225, but in steady state, under the power limit, 231
+// / 239 (1.50 / 1.34 GHz: memory-bound MMAs here cost more power); e4m3 cold
+// 141 / 120.
 static bool few_rows(int64_t P, int experts, bool e4m3) { return P <= 64 || (!e4m3 && P <= 2 * int64_t(experts)); }
 // Tens of rows (vx_grouped_mid.cu) / the tiles here, E = 512, N = 1,024: 10
-// rows an expert e4m3 178 / 179, 40 bf16 368 / 377, 80 e4m3 230 / 227; E = 64,
-// 128 rows 72 / 71, 640 158 / 150.  Banks of short rows (K = 512, N = 2,048)
+// rows an expert e4m3 176 / 177, 40 bf16 363 / 371, 80 e4m3 224 / 222; E = 64,
+// 128 rows 69.3 / 69.0, 640 158 / 150.  Banks of short rows (K = 512, N = 2,048)
 // e4m3 40 rows 98 / 146, 160 183 / 198; bf16 160 270 / 267.  It cuts a bank
 // into half as many tiles, so they have to be enough for the SMs: E = 8, 16
 // rows 21.7 / 18.9.

@@ -15,9 +15,9 @@
 // 256 columns and share the bank's rows.  The padding rows of X are not
 // copied; they hold what the ring held before, and their rows of D are not
 // read.  A tile of at most 64 positions takes M = 64: less power, and with it
-// higher clocks (2,048 tokens over 512 e4m3 experts in steady state 210 us,
-// 222 with M = 128 throughout).  Those 2,048 tokens: 199 us at full clocks for
-// 1.12 GB, 0.86 of the measured copy rate, the gathering of the rows included.
+// higher clocks (2,048 tokens over 512 e4m3 experts in steady state 206 us,
+// 219 with M = 128 throughout).  Those 2,048 tokens: 194 us at full clocks for
+// 1.12 GB, 0.88 of the measured copy rate, the gathering of the rows included.
 //
 // Warp roles (384 threads, one CTA an SM, persistent):
 //   warp 0      TMA: 256 bank rows (32 KB) and the real positions' rows (boxes
