@@ -24,7 +24,7 @@
 // writes its part of N.  B and y are on their way while h is being summed.
 //
 // Above: lora_group_kernel sorts the batch into items of 32 tokens,
-// lora_shrink_kernel (a CTA an item) writes h as bf16 pairs, and
+// lora_shrink_kernel (a CTA an item and 32 components) writes h as bf16 pairs, and
 // lora_expand_kernel (a CTA an item and 512 to 4,096 outputs) streams y.
 #include "vx_async.cuh"
 #include "vx_common.cuh"
@@ -125,13 +125,13 @@ VX_DEVICE int lora_rank(const LoraArgs& a, int e) {
 }
 
 // A_e x of the item's n tokens over the 32-input blocks first, first + stride,
-// ... of the CTA's warps, 8 * NT components at a time; out(row, r, v) gets
-// four neighbouring sums of the CTA.  part: the warps' sums, 128 MT NT floats
+// ... of the CTA's warps, 8 * NT components at a time, those from r_first,
+// r_first + r_step, ...; out(row, r, v) gets four neighbouring sums of the CTA.  part: the warps' sums, 128 MT NT floats
 // each.  AHEAD: the next block's operands are loaded before the present one's
 // MMAs.  ready() is called by every thread once, before the first out().
 template <int MT, int NT, bool AHEAD, typename G, typename F>
-VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, int n, int first, int stride,
-                           float* part, G&& ready, F&& out) {
+VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, int r_first, int r_step, const int* tok, int n,
+                           int first, int stride, float* part, G&& ready, F&& out) {
   constexpr int TM = 16 * MT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const uint16_t* xrow[2 * MT];
@@ -142,7 +142,7 @@ VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, i
   }
   const uint16_t* A = a.a + int64_t(e) * a.R * a.K;
   const int blocks = (a.K + 31) / 32;
-  for (int r0 = 0; r0 < rank; r0 += 8 * NT) {
+  for (int r0 = r_first; r0 < rank; r0 += r_step) {
     const int tiles = (min(8 * NT, rank - r0) + 7) / 8;
     float acc[MT][NT][4] = {};
     auto load = [&](int kb, uint4 (&xf)[2 * MT], uint4 (&af)[NT]) {
@@ -200,7 +200,7 @@ VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, const int* tok, i
       }
     }
     __syncthreads();
-    if (r0 == 0) ready();
+    if (r0 == r_first) ready();
     for (int i = tid; i < n * 2 * NT; i += kLoraThreads) {
       const int row = i / (2 * NT), col = i % (2 * NT) * 4;
       if (col >= tiles * 8) continue;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
     if (tid == 0) mbar_expect(smem_u32(&arrived), uint32_t(C * n * ((rank + 7) / 8) * 32));
     // the cluster barrier is a warp's, not a thread's: whole warps wait at it
     lora_shrink<1, kSmallNt, false>(
-        a, e, rank, tok, n, nb0, stride, part, [] { lora_cluster_wait(); },
+        a, e, rank, 0, 8 * kSmallNt, tok, n, nb0, stride, part, [] { lora_cluster_wait(); },
         [&](int row, int r, float4 v) {
           for (int q = 0; q < C; ++q) push4(parts + (cta * TM + row) * a.R + r, &arrived, q, v);
         });
@@ -434,29 +434,34 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
 
 constexpr int kLargeMt = 2, kLargeTm = 16 * kLargeMt;
 constexpr int kLargeNt = 4, kLargeKb = 1;
+constexpr int kPassRank = 8 * kLargeNt;   // components a CTA forms at a time
 constexpr int kLargePart = kLoraWarps * kLargeTm * 8 * kLargeNt;   // floats
 
 // An item of lora_group_kernel: {adapter or -1, first place of `order`,
 // tokens (0: no item), rank}.
 
 // h [place of order][16 components][hi, lo][16] of every item.
+// A CTA forms 32 components of an item (neighbouring CTAs the others, over the
+// same x): 2,693 tokens of 51 adapters of rank 80, K = 3,352, 30 against 55 us
+// with the passes in a row, 8,192 of rank 64 52.5 against 53.2.
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const LoraArgs a,
                                                                       const int32_t* __restrict__ order,
                                                                       const int4* __restrict__ items,
-                                                                      uint16_t* __restrict__ h) {
+                                                                      uint16_t* __restrict__ h,
+                                                                      int passes) {
   chain_begin();
   __shared__ __align__(16) float part[kLargePart];
   __shared__ int tok[kLargeTm];
   const int tid = threadIdx.x;
-  const int4 it = __ldg(items + blockIdx.x);
-  const int e = it.x, begin = it.y, n = it.z, rank = it.w;
-  if (n == 0 || rank == 0) return;
+  const int4 it = __ldg(items + blockIdx.x / passes);
+  const int e = it.x, begin = it.y, n = it.z, rank = it.w, first = int(blockIdx.x % passes) * kPassRank;
+  if (n == 0 || first >= rank) return;
   if (tid < kLargeTm) tok[tid] = tid < n ? __ldg(order + begin + tid) : -1;
   const float scale = a.scales ? __ldg(a.scales + e) : 1.0f;
   __syncthreads();
   const int pitch = ((a.R + 15) & ~15) * 2;
   lora_shrink<kLargeMt, kLargeNt, true>(
-      a, e, rank, tok, n, tid >> 5, kLoraWarps, part, [] {},
+      a, e, rank, first, passes * kPassRank, tok, n, tid >> 5, kLoraWarps, part, [] {},
       [&](int row, int r, float4 v) {
         const float f[4] = {v.x, v.y, v.z, v.w};
         uint16_t hi[4], lo[4];
@@ -692,6 +697,7 @@ static cudaError_t launch_lora_large(const LoraArgs& a, char* ws, cudaStream_t s
     const int64_t ctas = int64_t(n) * ((a.N + c - 1) / c), cost = (ctas + resident - 1) / resident * (c + 160);
     if (c == 512 || (4 * ctas >= 3 * resident && cost < best)) best = cost, cols = int(c);
   }
+  const unsigned passes = unsigned(a.R + kPassRank - 1) / kPassRank;
   static std::atomic<uint64_t> done{0};
   auto expand = lora_expand_kernel<WIDE>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(expand), lora_frag_bytes(kLargeMt, kLoraMaxRank), done);
@@ -699,7 +705,8 @@ static cudaError_t launch_lora_large(const LoraArgs& a, char* ws, cudaStream_t s
     e = launch_chained(lora_group_kernel, dim3(1), dim3(kGroupThreads), size_t(2 * a.L + 2) * sizeof(int), st, a,
                        place, order, items, int(n));
   if (e == cudaSuccess)
-    e = launch_chained(lora_shrink_kernel, dim3(n), dim3(kLoraThreads), 0, st, a, order, items, h);
+    e = launch_chained(lora_shrink_kernel, dim3(n * passes), dim3(kLoraThreads), 0, st, a, order, items, h,
+                       int(passes));
   if (e == cudaSuccess)
     e = launch_chained(expand, dim3(n, unsigned((a.N + cols - 1) / cols)), dim3(kLoraThreads),
                        size_t(lora_frag_bytes(kLargeMt, a.R)), st, a, order, items, h, cols);
