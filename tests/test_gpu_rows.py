@@ -166,3 +166,35 @@ def test_rows_on_another_stream_and_in_a_graph():
     for a in (gots, replays):
         for u, v in zip(a, wants):
             assert torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("residual", ["none", "bf16", "f32"])
+@pytest.mark.parametrize("T,d", [(3, 2), (3, 4), (5, 130), (5, 252), (700, 12), (3, 258), (3, 516), (2, 1002), (2, 1004),
+                                 (2, 8194), (1, 16388)])
+def test_norm_widths_that_four_or_two_divide(T, d, residual):
+    x = normal(50, T, d, spread=0.7)
+    res = None if residual == "none" else normal(51, T, d, spread=3.0,
+                                                 dtype=torch.bfloat16 if residual == "bf16" else torch.float32)
+    check_norm(x, res, 1 + normal(52, d, spread=0.2), 1e-6, "both", f"T={T} d={d} {residual}")
+
+
+@pytest.mark.parametrize("first", [1, 2, 4, 6, 8])
+def test_rows_that_start_between_vectors(first):
+    """One tensor's rows off the others' boundary: the narrowest one counts."""
+    T, d = 5, 256
+    x, res, gain = normal(53, T, d + 16), normal(54, T, d, dtype=torch.float32), normal(55, d + 16)
+    check_norm(x[:, first:first + d], res, 1 + gain[:d], 1e-6, "both", f"x from {first}")
+    check_norm(x[:, :d], None, (1 + gain)[first:first + d], 1e-6, "both", f"gain from {first}")
+    wide = normal(56, T, d + 16, dtype=torch.float32)
+    check_norm(x[:, :d], wide[:, first:first + d], 1 + gain[:d], 1e-6, "both", f"residual from {first}")
+    gate, up = normal(57, T, d + 16, spread=2.0), normal(58, T, d)
+    r = vxmoe.swiglu_e4m3(gate[:, first:first + d], up)
+    check_rows(swiglu64(gate[:, first:first + d], up), r.q, r.scales, f"gate from {first}")
+
+
+@pytest.mark.parametrize("P,width", [(3, 2), (5, 12), (600, 34), (4, 126), (4, 516), (3, 1002), (2, 8194), (1, 16388)])
+def test_swiglu_widths_that_four_or_two_divide(P, width):
+    both = normal(59, P, 2 * width, spread=2.0)
+    gate, up = both[:, :width], both[:, width:]
+    r = vxmoe.swiglu_e4m3(gate, up)
+    check_rows(swiglu64(gate, up), r.q, r.scales, f"{P}x{width}")

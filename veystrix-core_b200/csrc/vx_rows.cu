@@ -19,11 +19,12 @@
 //
 // Rows are dealt round robin to groups of threads, a warp (four groups a CTA)
 // or a CTA; a group has its next row's loads in flight while it reduces and
-// writes the present one.  V is the elements a load brings: 8 where every row
-// starts on a 16-byte boundary and the width is a multiple of 8, else 1.
+// writes the present one.  V is the elements an access takes: the largest of 8,
+// 4, 2 and 1 that divides the width and on whose boundary every row starts.
 // Rows too wide for the registers of 1,024 threads are read twice (LOOP).
 #include <cuda_fp8.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "vx_common.cuh"
@@ -72,32 +73,38 @@ VX_DEVICE float max_abs(float top, float v) {
 // V elements of a row as they lie in memory, and as float32.
 template <int V, typename E>
 struct Raw {
-  static constexpr int kWords = V * int(sizeof(E)) / 16;
-  uint4 w[kWords];
-  VX_DEVICE void load(const E* p) {
+  static constexpr int kWords = V * int(sizeof(E)) / 4;   // 32-bit words
+  uint32_t w[kWords];
+  template <bool AGAIN>
+  VX_DEVICE void read(const E* p) {
+    if constexpr (kWords % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = ldg_nc(reinterpret_cast<const uint4*>(p) + i);
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
+        const uint4 v = AGAIN ? __ldg(q) : ldg_nc(q);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    } else if constexpr (kWords == 2) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    }
   }
-  VX_DEVICE void load_again(const E* p) {   // what every row reads: kept in L1
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  }
+  VX_DEVICE void load(const E* p) { read<false>(p); }
+  VX_DEVICE void load_again(const E* p) { read<true>(p); }   // what every row reads: kept in L1
   VX_DEVICE void zero() {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
   VX_DEVICE void get(float (&f)[V]) const {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-      const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (sizeof(E) == 2) {
-          f[8 * i + 2 * j] = __uint_as_float(u[j] << 16);
-          f[8 * i + 2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
-        } else {
-          f[4 * i + j] = __uint_as_float(u[j]);
-        }
+      if (sizeof(E) == 2) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      } else {
+        f[i] = __uint_as_float(w[i]);
       }
     }
   }
@@ -116,14 +123,21 @@ VX_DEVICE void store_row(uint16_t* p, const float (&f)[V]) {
   if constexpr (V == 8)
     *reinterpret_cast<uint4*>(p) =
         make_uint4(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]), bf16x2(f[4], f[5]), bf16x2(f[6], f[7]));
+  else if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(p) = make_uint2(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]));
+  else if constexpr (V == 2)
+    *reinterpret_cast<uint32_t*>(p) = bf16x2(f[0], f[1]);
   else
     *p = uint16_t(bf16x2(f[0], 0.f));
 }
 template <int V>
 VX_DEVICE void store_row(float* p, const float (&f)[V]) {
-  if constexpr (V == 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4)
+      *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
   } else {
     *p = f[0];
   }
@@ -133,6 +147,10 @@ VX_DEVICE void store_row(uint8_t* p, const float (&f)[V]) {
   if constexpr (V == 8)
     *reinterpret_cast<uint2*>(p) = make_uint2(e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16),
                                               e4m3x2(f[4], f[5]) | (e4m3x2(f[6], f[7]) << 16));
+  else if constexpr (V == 4)
+    *reinterpret_cast<uint32_t*>(p) = e4m3x2(f[0], f[1]) | (e4m3x2(f[2], f[3]) << 16);
+  else if constexpr (V == 2)
+    *reinterpret_cast<uint16_t*>(p) = uint16_t(e4m3x2(f[0], f[1]));
   else
     *p = uint8_t(e4m3x2(f[0], 0.f));
 }
@@ -383,8 +401,24 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) swiglu_e4m3_kernel(
 
 // ---- host side --------------------------------------------------------------
 
-static bool starts_on(const void* p, int64_t ld, int64_t size, int64_t bytes) {
-  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * size % bytes == 0);
+// Rows p + i * ld of elements of `size` bytes (null: none).
+struct RowsAt {
+  const void* p;
+  int64_t ld, size;
+};
+// Elements an access may take: the largest of 8, 4, 2, 1 that divides the width
+// and on whose boundary every row starts.
+static int access_width(int width, std::initializer_list<RowsAt> all) {
+  int v = 8;
+  while (width % v) v /= 2;
+  for (const RowsAt& r : all) {
+    auto fits = [&] {
+      const int64_t bytes = v * r.size < 16 ? v * r.size : 16;
+      return !r.p || (reinterpret_cast<uintptr_t>(r.p) % bytes == 0 && r.ld * r.size % bytes == 0);
+    };
+    while (v > 1 && !fits()) v /= 2;
+  }
+  return v;
 }
 
 // Registers a thread of `kernel` uses (a property of the code: looked up once).
@@ -411,9 +445,8 @@ static unsigned row_ctas(int64_t groups, int threads, int registers) {
 // Calls f with the variant for rows of `width` elements (V, NV, one warp,
 // loop as integral constants), the groups and the threads of a CTA.
 template <typename F>
-static cudaError_t per_row_shape(bool wide, int64_t rows, int width, F&& f) {
+static cudaError_t per_row_shape(int v, int64_t rows, int width, F&& f) {
   using std::integral_constant;
-  const int v = wide ? 8 : 1;
   const int vecs = (width + v - 1) / v;
   auto run = [&](auto V, auto NV, auto W, auto L) {
     const int threads = W ? 128 : L ? 1024 : ((vecs + NV - 1) / NV + 31) / 32 * 32;
@@ -422,7 +455,7 @@ static cudaError_t per_row_shape(bool wide, int64_t rows, int width, F&& f) {
 #define VX_ROWS(V, NV, W, L)                                                                 \
   run(integral_constant<int, V>(), integral_constant<int, NV>(), integral_constant<bool, W>(), \
       integral_constant<bool, L>())
-  if (wide) {
+  if (v == 8) {
     if (vecs <= 32) return VX_ROWS(8, 1, true, false);
     // A batch that fills the GPU gives each row fewer threads with more loads
     // each, one warp where the registers allow (no CTA barrier): norm 65,536 x
@@ -436,9 +469,10 @@ static cudaError_t per_row_shape(bool wide, int64_t rows, int width, F&& f) {
     if (vecs <= 2048) return VX_ROWS(8, 2, false, false);
     return VX_ROWS(8, 1, false, true);
   }
-  if (vecs <= 128) return VX_ROWS(1, 4, true, false);
-  if (vecs <= 4096) return VX_ROWS(1, 4, false, false);
-  return VX_ROWS(1, 1, false, true);
+#define VX_NARROW(V)                                                                            \
+  (vecs <= 128 ? VX_ROWS(V, 4, true, false) : vecs <= 4096 ? VX_ROWS(V, 4, false, false) : VX_ROWS(V, 1, false, true))
+  return v == 4 ? VX_NARROW(4) : v == 2 ? VX_NARROW(2) : VX_NARROW(1);
+#undef VX_NARROW
 #undef VX_ROWS
 }
 
@@ -446,10 +480,9 @@ template <typename RES>
 static cudaError_t add_rmsnorm_as(const uint16_t* x, int64_t ldx, const RES* residual, int64_t ldr,
                                   const uint16_t* gain, int64_t T, int d, float eps, RES* residual_out,
                                   uint16_t* y, uint8_t* q, float* scales, cudaStream_t st) {
-  const bool wide = d % 8 == 0 && starts_on(x, ldx, 2, 16) && starts_on(residual, ldr, sizeof(RES), 16) &&
-                    starts_on(gain, 0, 2, 16) && starts_on(residual_out, d, sizeof(RES), 16) &&
-                    starts_on(y, d, 2, 16) && starts_on(q, d, 1, 8);
-  return per_row_shape(wide, T, d, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
+  const int access = access_width(d, {{x, ldx, 2}, {residual, ldr, sizeof(RES)}, {gain, 0, 2},
+                                      {residual_out, d, sizeof(RES)}, {y, d, 2}, {q, d, 1}});
+  return per_row_shape(access, T, d, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
     auto k = add_rmsnorm_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value, RES, decltype(l)::value>;
     static const int registers = registers_of(k);
     return launch_chained(k, dim3(row_ctas(groups, threads, registers)), dim3(threads), 0, st, x, ldx, residual, ldr,
@@ -471,9 +504,8 @@ cudaError_t launch_add_rmsnorm(const uint16_t* x, int64_t ldx, const void* resid
 cudaError_t launch_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_t ldu, int64_t rows,
                                int width, uint8_t* q, float* scales, cudaStream_t st) {
   if (rows == 0) return cudaSuccess;
-  const bool wide = width % 8 == 0 && starts_on(gate, ldg, 2, 16) && starts_on(up, ldu, 2, 16) &&
-                    starts_on(q, width, 1, 8);
-  return per_row_shape(wide, rows, width, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
+  const int access = access_width(width, {{gate, ldg, 2}, {up, ldu, 2}, {q, width, 1}});
+  return per_row_shape(access, rows, width, [&](auto v, auto nv, auto w, auto l, int64_t groups, int threads) {
     auto k = swiglu_e4m3_kernel<decltype(v)::value, decltype(nv)::value, decltype(w)::value, decltype(l)::value>;
     static const int registers = registers_of(k);
     return launch_chained(k, dim3(row_ctas(groups, threads, registers)), dim3(threads), 0, st, gate, ldg, up, ldu, rows,
