@@ -198,3 +198,22 @@ def test_swiglu_widths_that_four_or_two_divide(P, width):
     gate, up = both[:, :width], both[:, width:]
     r = vxmoe.swiglu_e4m3(gate, up)
     check_rows(swiglu64(gate, up), r.q, r.scales, f"{P}x{width}")
+
+
+@pytest.mark.parametrize("width", [201, 402, 612, 401, 802, 777, 1554, 1187, 2374])
+def test_many_rows_of_narrow_accesses(width):
+    """Enough rows that each takes one warp or few threads, several accesses a thread."""
+    T = 2401
+    x, res, gain = normal(60, T, width), normal(61, T, width, dtype=torch.float32), 1 + normal(62, width, spread=0.2)
+    res[7], x[7] = 0, 0
+    x[8, width - 1] = float("nan")
+    good = torch.arange(T, device="cuda") != 8
+    for residual in (res, res.bfloat16()):
+        r = vxmoe.add_rms_norm(x, residual, gain, 1e-6, output="both")
+        s, v = norm64(x, residual, gain, 1e-6)
+        within(r.y[good], v[good], v[good].abs() * (BF16 + 2 * ROW32), f"{width} y")
+        check_rows(v[good], r.q[good], r.scales[good], f"{width} q")
+        assert r.y[8].isnan().all() and r.scales[8].isnan()
+    both = normal(63, T, 2 * width, spread=2.0)
+    q = vxmoe.swiglu_e4m3(both[:, :width], both[:, width:])
+    check_rows(swiglu64(both[:, :width], both[:, width:]), q.q, q.scales, f"swiglu {width}")

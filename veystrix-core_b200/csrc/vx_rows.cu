@@ -227,11 +227,27 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       for (int j = 0; j < V; ++j) sv[j] += r[j];
     }
   };
-  auto gains = [&](int i, float (&gv)[V]) {   // from L1: the same for every row
+  // The gains are the same for every row: from L1, or held where they take few
+  // registers (odd rows, whose accesses bring one or two elements).
+  constexpr bool kHeld = V <= 2 && !LOOP;
+  float held[kHeld ? NV : 1][V];
+  auto read_gains = [&](int i, float (&gv)[V]) {
     Raw<V, uint16_t> w;
     if (i < d) w.load_again(gain + i); else w.zero();
     w.get(gv);
   };
+  auto gains = [&](int i, int n, float (&gv)[V]) {
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) gv[j] = held[n][j];
+    } else {
+      read_gains(i, gv);
+    }
+  };
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) read_gains(i0 + n * step, held[n]);
+  }
   if (!LOOP && grp.row < T) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) fetch(grp.row, i0 + n * step, n);
@@ -246,7 +262,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
           float gv[V];
           fetch(t, i, 0);
           sum_of(0, s[0]);
-          gains(i, gv);
+          gains(i, 0, gv);
 #pragma unroll
           for (int j = 0; j < V; ++j) f(s[0][j], gv[j]);
         }
@@ -254,7 +270,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
           float gv[V];
-          gains(i0 + n * step, gv);
+          gains(i0 + n * step, n, gv);
 #pragma unroll
           for (int j = 0; j < V; ++j) f(s[n][j], gv[j]);
         }
@@ -300,9 +316,9 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
     const float2 sc = row_scale(top);
     if (scales && i0 == 0) scales[t] = sc.x;
 
-    auto write = [&](int i, float (&sv)[V]) {
+    auto write = [&](int i, int n, float (&sv)[V]) {
       float gv[V];
-      gains(i, gv);
+      gains(i, n, gv);
       if (residual_out) store_row<V>(residual_out + t * d + i, sv);
 #pragma unroll
       for (int j = 0; j < V; ++j) sv[j] = sv[j] * r * gv[j];
@@ -317,12 +333,12 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       for (int i = i0; i < d; i += step) {
         fetch(t, i, 0);
         sum_of(0, s[0]);
-        write(i, s[0]);
+        write(i, 0, s[0]);
       }
     } else {
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        if (i0 + n * step < d) write(i0 + n * step, s[n]);
+        if (i0 + n * step < d) write(i0 + n * step, n, s[n]);
     }
   }
 }
@@ -455,19 +471,30 @@ static cudaError_t per_row_shape(int v, int64_t rows, int width, F&& f) {
 #define VX_ROWS(V, NV, W, L)                                                                 \
   run(integral_constant<int, V>(), integral_constant<int, NV>(), integral_constant<bool, W>(), \
       integral_constant<bool, L>())
+  const bool many = rows >= 4 * int64_t(sm_count());
   if (v == 8) {
     if (vecs <= 32) return VX_ROWS(8, 1, true, false);
     // A batch that fills the GPU gives each row fewer threads with more loads
     // each, one warp where the registers allow (no CTA barrier): norm 65,536 x
     // 512 52 against 60 us, swiglu 20,480 x 1,024 18.8 against 21.6 us; a
     // smaller batch spreads its rows: norm 64 x 2,048 2.1 us either way.
-    const bool many = rows >= 4 * int64_t(sm_count());
     if (many && vecs <= 64) return VX_ROWS(8, 2, true, false);
     if (many && vecs <= 96) return VX_ROWS(8, 3, true, false);
     if (many && vecs <= 128) return VX_ROWS(8, 4, true, false);
     if (vecs <= 1024 && !many) return VX_ROWS(8, 1, false, false);
     if (vecs <= 2048) return VX_ROWS(8, 2, false, false);
     return VX_ROWS(8, 1, false, true);
+  }
+  // The same with narrower accesses: a warp up to 32 of them a lane, then more
+  // a thread.  Norm 20,000 x 555 36 against 50 us, 13,012 x 1,187 51 / 68, 8,192 x
+  // 1,004 15.2 / 14.7; swiglu 47,605 x 413 25 / 52, 20,000 x 777 21 / 42, 20,000 x
+  // 996 17 / 21, 4,000 x 4,002 21 / 25.
+  if (v == 4 && many && vecs > 128 && vecs <= 256) return VX_ROWS(4, 8, true, false);
+  if (v <= 2 && many && vecs > 128 && vecs <= 8192) {
+    if (vecs <= 256) return v == 2 ? VX_ROWS(2, 8, true, false) : VX_ROWS(1, 8, true, false);
+    if (vecs <= 512) return v == 2 ? VX_ROWS(2, 16, true, false) : VX_ROWS(1, 16, true, false);
+    if (vecs <= 1024) return v == 2 ? VX_ROWS(2, 32, true, false) : VX_ROWS(1, 32, true, false);
+    return v == 2 ? VX_ROWS(2, 8, false, false) : VX_ROWS(1, 8, false, false);
   }
 #define VX_NARROW(V)                                                                            \
   (vecs <= 128 ? VX_ROWS(V, 4, true, false) : vecs <= 4096 ? VX_ROWS(V, 4, false, false) : VX_ROWS(V, 1, false, true))
