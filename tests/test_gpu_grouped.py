@@ -290,3 +290,24 @@ def test_two_streams_and_two_graphs_at_once():
     torch.cuda.synchronize()
     for got in outs + eager:
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("K", [256, 576])
+@pytest.mark.parametrize("counts", [[100], [5, 128, 127, 66], [17] * 12, [300, 0, 1000, 33]],
+                         ids=lambda c: "-".join(map(str, c[:4])))
+@pytest.mark.parametrize("N", [4, 12, 20, 131, 258, 260, 268, 304])
+def test_stores_of_every_width(kind, K, counts, N):
+    """Short bank rows (the positions-as-M tiles) and longer ones; outputs whose rows
+    16, 4, 2 or 1 elements divide, with and without neighbours in the same row."""
+    P = sum(counts)
+    x, w, xs, ws = operands(kind, P, len(counts), N, K, seed=31)
+    offsets = offsets_of(counts)
+    what = f"{kind} {counts} {N}x{K}"
+    clean = check(x, w, offsets, what, x_scales=xs, w_scales=ws)
+    for left, width in ((0, 320), (4, 324), (3, 331)):
+        out = torch.full((P + 2, width), 5.0, dtype=torch.bfloat16, device="cuda")
+        got = vxmoe.grouped_matmul(x, w, offsets, x_scales=xs, w_scales=ws, out=out[1:P + 1, left:left + N])
+        assert torch.equal(got.contiguous().view(torch.int16), clean.view(torch.int16)), f"{what} from {left}"
+        out[1:P + 1, left:left + N] = 5
+        assert bool((out == 5).all()), f"{what}: something beside the outputs was written"

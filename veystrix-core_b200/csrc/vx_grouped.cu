@@ -435,13 +435,15 @@ bool encode_k_rows(CUtensorMap* m, const void* p, bool fp8, int64_t K, int64_t r
 static bool few_rows(int64_t P, int experts, bool e4m3) { return P <= 64 || (!e4m3 && P <= 2 * int64_t(experts)); }
 // Tens of rows (vx_grouped_mid.cu) / the tiles here, E = 512, N = 1,024: 10
 // rows an expert e4m3 176 / 177, 40 bf16 363 / 371, 80 e4m3 224 / 222; E = 64,
-// 128 rows 69.3 / 69.0, 640 158 / 150.  Banks of short rows (K = 512, N = 2,048)
-// e4m3 40 rows 98 / 146, 160 183 / 198; bf16 160 270 / 267.  It cuts a bank
-// into half as many tiles, so they have to be enough for the SMs: E = 8, 16
-// rows 21.7 / 18.9.
+// 128 rows 69.3 / 69.0, 640 158 / 150.  Banks of short rows are stores first,
+// which are wider there: K = 512 e4m3, N = 2,048 40 rows 98 / 146, 160 183 /
+// 198, E = 1 and 20,000 rows 37 / 45; K = 256 bf16 E = 8 and 2,048 rows 27 /
+// 36, E = 4 and 500 7.2 / 9.0; K = 512 bf16, N = 2,048 160 rows 270 / 267.  It
+// cuts a bank into half as many tiles, so with long rows they have to be
+// enough for the SMs: E = 8, 16 rows 21.7 / 18.9.
 static bool mid_rows(const GroupedArgs& a, int64_t row_bytes) {
   const int64_t groups = a.P < a.experts ? a.P : a.experts, tiles = groups * ((a.N + 255) / 256);
-  return (a.P <= 64 * int64_t(a.experts) || row_bytes <= 512) && tiles >= sm_count();
+  return row_bytes <= 512 || (a.P <= 64 * int64_t(a.experts) && tiles >= sm_count());
 }
 
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows) {

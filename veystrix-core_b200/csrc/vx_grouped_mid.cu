@@ -26,7 +26,7 @@
 //               the MMAs
 //   warps 4-11  epilogue: TMEM lane = position, column = output; a lane
 //               stores 16 neighbouring outputs at once (32 bytes) where out's
-//               rows allow it, else 4, or single ones by way of shared memory
+//               rows allow it, else lanes share rows, 4 or 1 outputs each
 // Rows are gathered by a launch of their own before (gather_rows_kernel).
 // Every wait is bounded as in vx_grouped.cu.
 #include <cudaTypedefs.h>
@@ -44,7 +44,7 @@ constexpr int kMidThreads = 384;
 constexpr int kMidStages = 4;
 constexpr int kMidBank = kMidOut * 128, kMidStage = kMidBank + kMidPos * 128;
 constexpr int kMidEpiWarps = 8;
-constexpr int kOddPitch = 9;   // words of 16 outputs in shared memory, one more for the banks
+constexpr int kPiecePitch = 9;   // words of 16 outputs in shared memory, one more for the banks
 
 struct GroupedMid {
   CUtensorMap tm_w, tm_x[4];   // x: boxes of 16, 32, 64 and 128 rows
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kMidStages], empty[kMidStages], acc_full[2], acc_empty[2];
   __shared__ __align__(16) float w_scale[FP8 ? kMidEpiWarps : 1][kMidOut / 2];   // an epilogue warp's outputs
-  __shared__ uint32_t odd_rows[kMidEpiWarps][32 * kOddPitch];
+  __shared__ uint32_t pieces[kMidEpiWarps][32 * kPiecePitch];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   const GroupedArgs& a = g.a;
@@ -236,31 +236,42 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
           uint32_t w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) w[j] = ok ? bf16_pair(v[2 * j], v[2 * j + 1]) : 0x7FFF7FFFu;   // else NaN
-          if (real) {
-            uint16_t* o = out + 16 * i;
-            if (g.vec == 16 && left >= 16) {
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "r"(w[0]), "r"(w[1]),
-                           "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+          if (g.vec == 16 && left >= 16) {
+            if (real)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 16 * i), "r"(w[0]),
+                           "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                            : "memory");
-            } else if (g.vec > 1) {
+          } else if (g.vec > 1 && rows < 32) {
+            if (real) {
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (4 * j < left) *reinterpret_cast<uint2*>(o + 4 * j) = make_uint2(w[2 * j], w[2 * j + 1]);
+                if (4 * j < left)
+                  *reinterpret_cast<uint2*>(out + 16 * i + 4 * j) = make_uint2(w[2 * j], w[2 * j + 1]);
             }
-          }
-          if (g.vec == 1) {
-            // odd rows: two rows an instruction, 16 neighbouring outputs each,
-            // by way of shared memory (a lane's own row is 32 sectors an
-            // instruction: 27 against 14 us for 2,008 rows of 766)
-            uint32_t* r = odd_rows[warp - 4] + lane * kOddPitch;
+          } else {
+            // through shared memory, neighbouring lanes to neighbouring pieces
+            // of a row: lanes that store their own rows are 32 sectors an
+            // instruction (30,502 rows of 2,596 172 against 80 us, 2,008 of 766
+            // 27 / 14).  Four outputs of 16 rows go out faster as they lie: 341
+            // groups of 7 rows of 1,324 44 / 26, of 24 43 / 29; of 55 44 / 47.
+            uint32_t* r = pieces[warp - 4] + lane * kPiecePitch;
 #pragma unroll
             for (int j = 0; j < 8; ++j) r[j] = w[j];
             __syncwarp();
             const int last = min(rows, c.count - quarter * rows);   // the warp's real positions
-            const uint16_t* from = reinterpret_cast<const uint16_t*>(odd_rows[warp - 4]) + (lane & 15);
-            uint16_t* to = a.out + int64_t(c.p0 + quarter * rows) * a.ldo + n0 + 16 * i + (lane & 15);
-            if ((lane & 15) < left)
-              for (int q = lane >> 4; q < last; q += 2) to[q * a.ldo] = from[q * 2 * kOddPitch];
+            uint16_t* to = a.out + int64_t(c.p0 + quarter * rows) * a.ldo + n0 + 16 * i;
+            if (g.vec > 1) {
+              const int piece = 4 * (lane & 3);
+              if (piece < left)
+                for (int q = lane >> 2; q < last; q += 8) {
+                  const uint32_t* from = pieces[warp - 4] + q * kPiecePitch + piece / 2;
+                  *reinterpret_cast<uint2*>(to + q * a.ldo + piece) = make_uint2(from[0], from[1]);
+                }
+            } else if ((lane & 15) < left) {
+              for (int q = lane >> 4; q < last; q += 2)
+                to[q * a.ldo + (lane & 15)] =
+                    reinterpret_cast<const uint16_t*>(pieces[warp - 4] + q * kPiecePitch)[lane & 15];
+            }
             __syncwarp();
           }
         }
