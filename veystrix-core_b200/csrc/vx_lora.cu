@@ -79,8 +79,16 @@ VX_DEVICE int lora_id(const LoraArgs& a, int64_t t) {
   return e >= 0 && e < a.L ? e : -1;
 }
 
-// Eight neighbouring values of a row of y, from column n on.  WIDE: 16-byte
-// aligned and n + 8 <= N.  y may be written in place, so no read-only path.
+// A lane's eight values of a row of y in a block of 32 outputs.  WIDE: eight
+// neighbours, 16-byte aligned.  Else value i is output 8 (i / 2) + 4 (i % 2) + c
+// for lane c of four, so that a load of four lanes is four neighbours (8,192
+// tokens x 2,047 outputs 103 us, 128 with eight neighbours a lane).  y may be
+// written in place, so no read-only path.
+template <bool WIDE>
+VX_DEVICE int first_of(int nb) {
+  return nb * 32 + (WIDE ? 8 : 1) * int(threadIdx.x & 3);
+}
+VX_DEVICE int narrow_at(int n, int i) { return n + 8 * (i >> 1) + 4 * (i & 1); }
 template <bool WIDE>
 struct Eight {
   uint32_t w[WIDE ? 4 : 8];
@@ -92,7 +100,7 @@ struct Eight {
                    : "memory");
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = n + i < N ? uint32_t(row[n + i]) << 16 : 0u;
+      for (int i = 0; i < 8; ++i) w[i] = narrow_at(n, i) < N ? uint32_t(row[narrow_at(n, i)]) << 16 : 0u;
     }
   }
   VX_DEVICE float get(int i) const {
@@ -113,7 +121,7 @@ VX_DEVICE void store8(uint16_t* row, int n, int N, const float (&v)[8]) {
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (n + i < N) row[n + i] = uint16_t(lora_bf16x2(v[i], 0.f));
+      if (narrow_at(n, i) < N) row[narrow_at(n, i)] = uint16_t(lora_bf16x2(v[i], 0.f));
   }
 }
 
@@ -232,17 +240,17 @@ VX_DEVICE int lora_frag_at(int row, int r) {
   return ((kb * MT + (row >> 4)) * 64 + lane) * 8 + reg * 2 + (r & 1);
 }
 
-// B of one 32-output block: KB pairs of 16 components x 4 MMA tiles.
-// Column q of MMA tile j is output 8 (q/2) + 2 j + q%2 of the 32, so a lane
-// ends up with 8 neighbours.
-template <int KB>
+// B of one 32-output block: KB pairs of 16 components x 4 MMA tiles.  Column q
+// of MMA tile j is output 8 (q/2) + 2 j + q%2 of the 32, so a lane ends up with
+// 8 neighbours; not WIDE 8 j + 4 (q%2) + q/2 (Eight).
+template <int KB, bool WIDE>
 VX_DEVICE void load_b(const LoraArgs& a, const uint16_t* B, int rank, int nb, int kb0, uint4 (&bf)[KB][4]) {
   const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
 #pragma unroll
   for (int u = 0; u < KB; ++u) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = nb * 32 + 8 * (g >> 1) + 2 * j + (g & 1), r = (kb0 + u) * 32 + 8 * c;
+      const int row = nb * 32 + (WIDE ? 8 * (g >> 1) + 2 * j + (g & 1) : 8 * j + 4 * (g & 1) + (g >> 1)), r = (kb0 + u) * 32 + 8 * c;
       bf[u][j] = r < rank && row < a.N ? __ldg(reinterpret_cast<const uint4*>(B + int64_t(row) * a.R + r))
                                        : make_uint4(0, 0, 0, 0);
     }
@@ -250,7 +258,7 @@ VX_DEVICE void load_b(const LoraArgs& a, const uint16_t* B, int rank, int nb, in
 }
 template <int MT, bool WIDE>
 VX_DEVICE void load_y(const LoraArgs& a, const int (&t)[2 * MT], int nb, Eight<WIDE> (&y)[2 * MT]) {
-  const int n = nb * 32 + 8 * (threadIdx.x & 3);
+  const int n = first_of<WIDE>(nb);
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i)
     if (t[i] >= 0 && (!WIDE || n < a.N)) y[i].load(a.y + t[i] * a.ldy, n, a.N);
@@ -259,10 +267,10 @@ VX_DEVICE void load_y(const LoraArgs& a, const int (&t)[2 * MT], int nb, Eight<W
 template <int MT, int KB, bool WIDE>
 VX_DEVICE void lora_expand(const LoraArgs& a, const uint16_t* B, int rank, const uint4* frag, const int (&t)[2 * MT],
                            int nb, const Eight<WIDE> (&y)[2 * MT], uint4 (&bf)[KB][4]) {
-  const int lane = threadIdx.x & 31, c = lane & 3, n = nb * 32 + 8 * c, kbs = (rank + 31) / 32;
+  const int lane = threadIdx.x & 31, c = lane & 3, n = first_of<WIDE>(nb), kbs = (rank + 31) / 32;
   float acc[MT][4][4] = {};
   for (int kb0 = 0; kb0 < kbs; kb0 += KB) {
-    if (kb0 > 0) load_b<KB>(a, B, rank, nb, kb0, bf);
+    if (kb0 > 0) load_b<KB, WIDE>(a, B, rank, nb, kb0, bf);
 #pragma unroll
     for (int u = 0; u < KB; ++u) {
       if (kb0 + u >= kbs) break;
@@ -316,7 +324,7 @@ VX_DEVICE void lora_expand_all(const LoraArgs& a, const uint16_t* B, int rank, c
     int next = nb + stride;
     if (next * 32 < end) {
       load_y<MT, WIDE>(a, t, next, yn);
-      load_b<KB>(a, B, rank, next, 0, bn);
+      load_b<KB, WIDE>(a, B, rank, next, 0, bn);
     }
     lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, y, bf);
     nb = next;
@@ -324,7 +332,7 @@ VX_DEVICE void lora_expand_all(const LoraArgs& a, const uint16_t* B, int rank, c
     next = nb + stride;
     if (next * 32 < end) {
       load_y<MT, WIDE>(a, t, next, y);
-      load_b<KB>(a, B, rank, next, 0, bf);
+      load_b<KB, WIDE>(a, B, rank, next, 0, bf);
     }
     lora_expand<MT, KB, WIDE>(a, B, rank, frag, t, nb, yn, bn);
     nb = next;
@@ -410,7 +418,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
   }
   if (nb0 * 32 < a.N) {
     load_y<1, WIDE>(a, t, nb0, y);
-    load_b<kSmallKb>(a, B, rank, nb0, 0, bf);
+    load_b<kSmallKb, WIDE>(a, B, rank, nb0, 0, bf);
   }
   if (rank > 0) {
     const bool ok = lora_wait(&arrived);
@@ -473,8 +481,10 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_shrink_kernel(const Lora
       });
 }
 
+// Not WIDE one CTA an SM: with two its registers spill (2,000 tokens x 1,001
+// outputs 23 / 30 us, 8,192 x 2,047 103 / 99).
 template <bool WIDE>
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const LoraArgs a,
+__global__ void __launch_bounds__(kLoraThreads, WIDE ? 2 : 1) lora_expand_kernel(const LoraArgs a,
                                                                       const int32_t* __restrict__ order,
                                                                       const int4* __restrict__ items,
                                                                       const uint16_t* __restrict__ h, int cols) {
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_expand_kernel(const Lora
   Eight<WIDE> y[2 * kLargeMt];
   uint4 bf[kLargeKb][4];
   if (nb0 * 32 < end) {
-    load_b<kLargeKb>(a, B, rank, nb0, 0, bf);
+    load_b<kLargeKb, WIDE>(a, B, rank, nb0, 0, bf);
     load_y<kLargeMt, WIDE>(a, t, nb0, y);
   }
   // the fragments: a thread brings 4 components of a row, hi or lo.  What
