@@ -149,3 +149,13 @@ def test_two_streams_and_two_graphs_at_once():
     for got in (outs, eager):
         for g, v in zip(got, want):
             assert torch.equal(g, v)
+
+
+@pytest.mark.parametrize("N", [2048, 4096, 4093, 4104])
+def test_large_batches_and_wide_outputs(N):
+    """Enough items that a CTA takes up to 4,096 outputs, ranks of more than one pass, in place too."""
+    y, x, a, b, ids = operands(8200, 64, N, 3, 72, seed=71)
+    ranks = torch.tensor([72, 33, 8], device="cuda", dtype=torch.int32)
+    got = check(y, x, a, b, ids, f"N={N}", ranks=ranks)
+    vxmoe.lora_add(y, x, a, b, ids, ranks=ranks, out=y)
+    assert torch.equal(got.view(torch.int16), y.view(torch.int16)), "in place"
