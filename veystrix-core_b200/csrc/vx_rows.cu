@@ -10,12 +10,13 @@
 //
 // The norm's factor r = 1/sqrt(...) is common to a row, so max |v| is
 // r * max |s_i * gain_i|: sum and maximum come from the same pass, and one
-// block reduction serves both.  Rows whose squares or products s * gain leave
-// the float32 range take a second one over scaled values, or the values
-// themselves.  Rows are bound by memory: a row's elements
-// are read once, stay in the registers of its threads (as float32) until the
-// reduction is done, and every output is written once.  The maximum keeps
-// NaN, so a NaN anywhere makes the row's scale NaN as the formula does.
+// block reduction serves both.  Rows whose squares leave the float32 range at
+// its upper end take a second one over scaled values, rows whose products s *
+// gain leave it one over the values themselves.  Rows are bound by memory: a
+// row's elements are read once, stay in the registers of its threads (as
+// float32) until the reduction is done, and every output is written once.  The
+// maximum keeps NaN, so a NaN anywhere makes the row's scale NaN as the formula
+// does.
 //
 // Rows are dealt round robin to groups of threads, a warp (four groups a CTA)
 // or a CTA; a group has its next row's loads in flight while it reduces and
@@ -289,26 +290,29 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       top = max_abs(top, sv * gv);
     });
     row_reduce<ONE_WARP, true>(sum, top, turn);
-    float r;
+    // The norm's factor is pre * r; pre is 1 but for the rows below (all
+    // branches here are taken by whole rows).
+    float pre = 1.f;
     if (sum > kFloatMax) {
-      // the squares left the float32 range: the same on s / 2^70 (both
-      // branches are taken by whole rows)
+      // The squares left the float32 range: the same on s / 2^80.  s < 2^128, so
+      // its squares are below 2^96 and 2^29 of them below 2^125; the largest is
+      // at least 2^(128 - 29 - 160), so what drops below the range is nothing
+      // beside it.  eps 2^-160 is no constant: 2^-80 twice.
+      pre = 0x1p-80f;
       sum = 0.f;
       float unused = 0.f;
       each([&](float sv, float) {
-        sv *= 0x1p-70f;
+        sv *= pre;
         sum = fmaf(sv, sv, sum);
       });
       row_reduce<ONE_WARP, true>(sum, unused, turn);
-      r = __fdiv_rn(0x1p-70f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps * 0x1p-140f)));
-    } else {
-      r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps)));
     }
-    if (scales && !(top <= kFloatMax && top >= 0x1p-100f)) {
-      // some |s g| is no finite number, or all are below 2^-100 and lose bits:
-      // the maximum of the values themselves
+    const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps * pre * pre)));
+    if (scales && !(pre == 1.f && top <= kFloatMax && top >= 0x1p-100f)) {
+      // some |s g| is no finite number, or all are below 2^-100 and lose bits, or
+      // s is scaled: the maximum of the values themselves
       top = 0.f;
-      each([&](float sv, float gv) { top = max_abs(top, sv * r * gv); });
+      each([&](float sv, float gv) { top = max_abs(top, sv * pre * r * gv); });
       row_reduce<ONE_WARP, false>(sum, top, turn);
     } else {
       top *= r;   // max|v| up to the rounding of one product
@@ -320,6 +324,10 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       float gv[V];
       gains(i, n, gv);
       if (residual_out) store_row<V>(residual_out + t * d + i, sv);
+      if (pre != 1.f) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sv[j] *= pre;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) sv[j] = sv[j] * r * gv[j];
       if (y) store_row<V>(y + t * d + i, sv);
