@@ -50,3 +50,30 @@ def test_squares_above_the_range(T, d):
         for res in residuals(1, T, d, big / 16):
             check(x, res, gain, 1e-6, f"T={T} d={d} {big:.0e}")
             check(x, res, gain, 1e36, f"T={T} d={d} {big:.0e} and a large eps")
+
+
+@pytest.mark.parametrize("T", [3, 700])
+@pytest.mark.parametrize("d", WIDTHS)
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -149, 2.0 ** -120, 2.0 ** -101, 2.0 ** -99, 1e-6])
+def test_squares_below_the_range(T, d, eps):
+    gain = (1 + 0.1 * torch.randn(d, device="cuda", generator=gen(3))).bfloat16()
+    wide = gain * 2.0 ** 90
+    for power in (-55, -64, -70, -76, -90, -120, -126, -131):
+        x = (torch.randn((T, d), device="cuda", generator=gen(4)) * 2.0 ** power).bfloat16()
+        for res in residuals(5, T, d, 2.0 ** (power - 1)):
+            check(x, res, gain, eps, f"T={T} d={d} 2^{power} eps={eps}")
+        check(x, None, wide, eps, f"T={T} d={d} 2^{power} eps={eps} large gains")
+
+
+@pytest.mark.parametrize("d", WIDTHS)
+def test_rows_of_zeros_beside_small_ones(d):
+    x = torch.zeros((4, d), device="cuda", dtype=torch.bfloat16)
+    x[1, d - 1] = 2.0 ** -133          # the smallest bf16
+    x[2] = 2.0 ** -80
+    gain = torch.ones(d, device="cuda", dtype=torch.bfloat16)
+    r = vxmoe.add_rms_norm(x, None, gain, 0.0, output="both")
+    # 0 / 0, as the formula gives it
+    assert r.y[[0, 3]].float().isnan().all() and r.scales[[0, 3]].isnan().all()
+    check(x[1:3], None, gain, 0.0, "small rows")
+    r = vxmoe.add_rms_norm(x, None, gain, 1e-6, output="both")
+    assert not r.y[[0, 3]].float().any() and bool((r.scales[[0, 3]] == 2.0 ** -126).all())

@@ -11,7 +11,7 @@
 // The norm's factor r = 1/sqrt(...) is common to a row, so max |v| is
 // r * max |s_i * gain_i|: sum and maximum come from the same pass, and one
 // block reduction serves both.  Rows whose squares leave the float32 range at
-// its upper end take a second one over scaled values, rows whose products s *
+// either end take a second one over scaled values, rows whose products s *
 // gain leave it one over the values themselves.  Rows are bound by memory: a
 // row's elements are read once, stay in the registers of its threads (as
 // float32) until the reduction is done, and every output is written once.  The
@@ -294,11 +294,18 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
     // branches here are taken by whole rows).
     float pre = 1.f;
     if (sum > kFloatMax) {
-      // The squares left the float32 range: the same on s / 2^80.  s < 2^128, so
+      // The squares left the range upwards: the same on s / 2^80.  s < 2^128, so
       // its squares are below 2^96 and 2^29 of them below 2^125; the largest is
       // at least 2^(128 - 29 - 160), so what drops below the range is nothing
-      // beside it.  eps 2^-160 is no constant: 2^-80 twice.
+      // beside it.
       pre = 0x1p-80f;
+    } else if (sum < 0x1p-100f && eps < 0x1p-100f) {
+      // Squares may have lost bits or become zero (2^-150 each, which is nothing
+      // beside a sum of 2^-100, nor their mean's error beside such an eps): on
+      // 2^100 s, below 2^50, the least of them 2^-49.
+      pre = 0x1p100f;
+    }
+    if (pre != 1.f) {
       sum = 0.f;
       float unused = 0.f;
       each([&](float sv, float) {
@@ -307,6 +314,7 @@ __global__ void __launch_bounds__(ONE_WARP ? 128 : 1024) add_rmsnorm_kernel(
       });
       row_reduce<ONE_WARP, true>(sum, unused, turn);
     }
+    // eps pre^2 in two steps: pre^2 alone is no float32
     const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(d)), eps * pre * pre)));
     if (scales && !(pre == 1.f && top <= kFloatMax && top >= 0x1p-100f)) {
       // some |s g| is no finite number, or all are below 2^-100 and lose bits, or
