@@ -54,16 +54,18 @@ VX_DEVICE uint32_t bf16x2(float lo, float hi) {
 }
 
 // g / (1 + exp(-g)) * u.  With e = exp(-|g|) <= 1 the denominator stays in
-// [1, 2] and nothing overflows; e is the square of 2^(-|g| log2(e) / 2),
-// which no |g| whose e counts takes out of the normal range, so the
-// flush-to-zero exponential serves (half the instructions of the one that
-// keeps subnormals).  Off by a few 2^-22 and |g| 2^-24 of e.
+// [1, 2] and nothing overflows.  e is the square of h = 2^(-|g| log2(e) / 2); a
+// negative g's factor e goes in as two factors h, one at g and one at u: e alone
+// leaves the normal range at g = -87, h at -174, where the product is below
+// 2^-115 whatever u is (and counts as zero).  So the flush-to-zero exponential
+// serves (half the instructions of the one that keeps subnormals).  Off by a
+// few 2^-22, and by |g| 2^-23 of e.
 VX_DEVICE float swiglu_f32(float g, float u) {
   float h, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(g) * -0.72134752f));
-  const float e = h * h;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * (g < 0.f ? e : 1.0f) * r * u;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
+  const float f = g < 0.f ? h : 1.0f;
+  return g * f * r * (u * f);
 }
 // The larger of top and |v|, NaN if one of them is.
 VX_DEVICE float max_abs(float top, float v) {
