@@ -301,7 +301,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
       const int cols = c.count(h), p0 = c.first(h);
       const int n = c.row0 + int(rank) * 128 + quarter * 32 + lane;   // this lane's output
       const float sw = next.sw;
+      bool fit = true;
       if (FP8) {
+        fit = products_fit(next.sx, sw);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < kGtCols / 64; ++i) scale[32 * i + lane] = next.sx[i];
@@ -321,12 +323,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         if (c0 >= cols) break;
         float v[16];
         tmem_ld16(acc + c0, v);
-        if (FP8) {
+        if (FP8 && fit) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float4 f = *reinterpret_cast<const float4*>(scale + c0 + 4 * j);
             v[4 * j] *= f.x * sw, v[4 * j + 1] *= f.y * sw, v[4 * j + 2] *= f.z * sw, v[4 * j + 3] *= f.w * sw;
           }
+        } else if (FP8) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = scaled(v[j], scale[c0 + j], sw);
         }
         if (!ok) {
 #pragma unroll

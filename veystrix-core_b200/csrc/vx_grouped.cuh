@@ -131,6 +131,37 @@ struct GroupTable {
   }
 };
 
+// v * a * b for the two scales of a value.  Their product in one where that is a
+// normal number; where it would overflow or lose bits below 2^-126 although
+// the value does not, they enter one by one: below, the larger first (v is a
+// sum of e4m3 products, 2^-18 to 2^48: v times it stays in range), above, the
+// smaller.  A zero enters first.
+VX_DEVICE bool is_normal(float p) { return fabsf(p) >= 0x1p-126f && fabsf(p) <= 0x1.fffffep127f; }
+VX_DEVICE float scaled(float v, float a, float b) {
+  const float p = a * b;
+  if (is_normal(p)) return v * p;
+  const bool first = fabsf(a) > fabsf(b);
+  const float hi = first ? a : b, lo = first ? b : a;
+  return fabsf(p) < 1.f && lo != 0.f ? v * hi * lo : v * lo * hi;
+}
+// Whether v * (a * b) does for every scale a of the warp (N a lane, in s) and
+// every lane's b: no product of theirs that is neither zero nor normal.  One
+// check a tile, so that the tiles' inner loops multiply by the product.
+template <int N>
+VX_DEVICE bool products_fit(const float (&s)[N], float b) {
+  uint32_t hi = 0, lo = 0x7F800000u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t m = __float_as_uint(fabsf(s[i]));   // ordered as their values, NaN on top
+    hi = max(hi, m);
+    if (m) lo = min(lo, m);
+  }
+  hi = __reduce_max_sync(0xFFFFFFFFu, hi), lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+  const float m = fabsf(b);
+  return __all_sync(0xFFFFFFFFu, m * __uint_as_float(hi) <= 0x1.fffffep127f &&
+                                     (m == 0.f || m * __uint_as_float(lo) >= 0x1p-126f));
+}
+
 // True in one lane, the same one in every call, of a converged warp.  MMAs
 // issued under it in a loop that the whole warp runs keep their operands in
 // uniform registers; under `lane == 0` the compiler moves them there one by

@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(S)) grouped_few_kernel(c
     auto finish = [&](float v, int n, int pos) {
       if (FP8) {
         const int p = p0 + pos, row = a.rows ? row_of(a, p) : p;
-        v *= (row >= 0 ? __ldg(a.x_scales + row) : 0.f) * __ldg(a.w_scales + int64_t(e) * a.N + n);
+        v = scaled(v, row >= 0 ? __ldg(a.x_scales + row) : 0.f, __ldg(a.w_scales + int64_t(e) * a.N + n));
       }
       a.out[int64_t(p0 + pos) * a.ldo + n] = f32_to_bf16(v);
     };

@@ -205,14 +205,18 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
       const int rows = c.m() / 4, pos = quarter * rows + lane, n0 = c.n0 + h * (kMidOut / 2);
       const bool real = lane < rows && pos < c.count;
       float sx = 1.f;
+      bool fit = true;
       if (FP8) {
+        float sw[4];
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int n = n0 + 32 * i + lane;
-          scale[32 * i + lane] = n < a.N ? __ldg(a.w_scales + int64_t(c.e) * a.N + n) : 0.f;
+          sw[i] = n < a.N ? __ldg(a.w_scales + int64_t(c.e) * a.N + n) : 0.f;
+          scale[32 * i + lane] = sw[i];
         }
         if (real) sx = __ldg(a.x_scales + c.p0 + pos);
+        fit = products_fit(sw, sx);
         __syncwarp();
       }
       if (ok) ok = role_wait(smem_u32(&acc_full[b]), ph, &dead);
@@ -226,12 +230,15 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
           if (left <= 0) break;
           float v[16];
           tmem_ld16(tmem + lanes + b * kMidOut + h * (kMidOut / 2) + 16 * i, v);
-          if (FP8) {
+          if (FP8 && fit) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float4 f = *reinterpret_cast<const float4*>(scale + 16 * i + 4 * j);
               v[4 * j] *= f.x * sx, v[4 * j + 1] *= f.y * sx, v[4 * j + 2] *= f.z * sx, v[4 * j + 3] *= f.w * sx;
             }
+          } else if (FP8) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = scaled(v[j], scale[16 * i + j], sx);
           }
           uint32_t w[8];
 #pragma unroll
