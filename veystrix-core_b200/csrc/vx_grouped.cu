@@ -158,7 +158,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     grouped_kernel(const __grid_constant__ GroupedTc g) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kGtStages], empty[kGtStages], acc_full[2], acc_empty[2];
-  __shared__ __align__(16) float x_scale[FP8 ? kGtEpiWarps : 1][kGtCols / 2];   // an epilogue warp's columns
+  __shared__ __align__(16) float x_scale[kGtEpiWarps][kGtCols / 2];   // an epilogue warp's columns
   __shared__ uint32_t tmem_slot;
   __shared__ int dead;
   const GroupedArgs& a = g.a;
@@ -275,7 +275,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     // ---- epilogue: warp = a quarter of the outputs, half h of the positions
     const int quarter = warp & 3, h = (warp - 4) >> 2;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    float* scale = x_scale[FP8 ? warp - 4 : 0];
+    float* scale = x_scale[warp - 4];
     const uint32_t pick = lane & 1 ? 0x3276u : 0x5410u;
     int b = 0;
     uint32_t ph = 0;
@@ -288,9 +288,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     auto fetch = [&](int t) {
       if (t >= tiles) return;
       next.c = tile_at(t);
-      if (!FP8) return;
+      if (!FP8 && !a.gathered) return;
       const int n = next.c.row0 + int(rank) * 128 + quarter * 32 + lane;
-      next.sw = n < a.N ? __ldg(a.w_scales + int64_t(next.c.e) * a.N + n) : 0.f;
+      next.sw = FP8 && n < a.N ? __ldg(a.w_scales + int64_t(next.c.e) * a.N + n) : 0.f;
 #pragma unroll
       for (int i = 0; i < kGtCols / 64; ++i)
         next.sx[i] = 32 * i + lane < next.c.count(h) ? __ldg(a.x_scales + next.c.first(h) + 32 * i + lane) : 0.f;
@@ -301,8 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
       const int cols = c.count(h), p0 = c.first(h);
       const int n = c.row0 + int(rank) * 128 + quarter * 32 + lane;   // this lane's output
       const float sw = next.sw;
-      bool fit = true;
-      if (FP8) {
+      bool fit = true;   // no column's or output's scale, and no column, out of the ordinary
+      if (FP8 || a.gathered) {
         fit = products_fit(next.sx, sw);
         __syncwarp();
 #pragma unroll
@@ -329,9 +329,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
             const float4 f = *reinterpret_cast<const float4*>(scale + c0 + 4 * j);
             v[4 * j] *= f.x * sw, v[4 * j + 1] *= f.y * sw, v[4 * j + 2] *= f.z * sw, v[4 * j + 3] *= f.w * sw;
           }
-        } else if (FP8) {
+        } else if (!fit) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = scaled(v[j], scale[c0 + j], sw);
+          for (int j = 0; j < 16; ++j) {
+            const float f = scale[c0 + j];
+            v[j] = names_none(a, f) ? 0.f : FP8 ? scaled(v[j], f, sw) : v[j];
+          }
         }
         if (!ok) {
 #pragma unroll
@@ -373,10 +376,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
 
 // ---- rows gathered first ------------------------------------------------------
 
-// x row of every position (zeros where it lies outside x), and its scale.  A
-// warp copies kGatherPiece bytes of a row, all of its loads at once: many
-// short warps hide the row number's latency better than fewer with several
-// rows each.  20,480 rows of 2,048 bytes take 10 us.
+// x row of every position (zeros where it lies outside x), and its scale (1 if
+// x has none, kNoRow outside x).  A warp copies kGatherPiece bytes of a row,
+// all of its loads at once: many short warps hide the row number's latency
+// better than fewer with several rows each.  20,480 rows of 2,048 bytes take
+// 10 us.
 constexpr int kGatherThreads = 256, kGatherAhead = 4, kGatherPiece = kGatherAhead * 512;
 
 __global__ void __launch_bounds__(kGatherThreads) gather_rows_kernel(const GroupedArgs a, int row_bytes,
@@ -388,7 +392,10 @@ __global__ void __launch_bounds__(kGatherThreads) gather_rows_kernel(const Group
   const int64_t unit = int64_t(blockIdx.x) * (kGatherThreads / 32) + (threadIdx.x >> 5), p = unit / pieces;
   if (p >= a.P) return;
   const int from = int(unit - p * pieces) * kGatherPiece + lane * 16, row = row_of(a, int(p));
-  if (scales_out && from == 0) scales_out[p] = row < 0 ? 0.f : __ldg(a.x_scales + row);
+  if (from == 0) {
+    const float s = row >= 0 && a.x_scales ? __ldg(a.x_scales + row) : 1.f;
+    scales_out[p] = __uint_as_float(row < 0 ? kNoRow : s == s ? __float_as_uint(s) : 0x7FC00000u);
+  }
   const unsigned char* src = static_cast<const unsigned char*>(a.x) + (row < 0 ? 0 : row * ld_bytes);
   unsigned char* dst = rows_out + p * row_bytes;
   uint4 v[kGatherAhead];
@@ -454,7 +461,7 @@ static bool mid_rows(const GroupedArgs& a, int64_t row_bytes) {
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows) {
   if (!rows || few_rows(P, experts, e4m3)) return 0;
   const int64_t row = int64_t(K) * (e4m3 ? 1 : 2);
-  return ((P * row + 255) & ~int64_t(255)) + (e4m3 ? 4 * P : 0);
+  return ((P * row + 255) & ~int64_t(255)) + 4 * P;
 }
 
 // x and its scales in the order of the positions, in the workspace; a takes
@@ -462,7 +469,7 @@ int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool r
 static cudaError_t gather_rows(GroupedArgs& a, bool e4m3, void* workspace, cudaStream_t st) {
   const int size = e4m3 ? 1 : 2, row_bytes = a.K * size;
   unsigned char* rows = static_cast<unsigned char*>(workspace);
-  float* scales = e4m3 ? reinterpret_cast<float*>(rows + ((a.P * row_bytes + 255) & ~int64_t(255))) : nullptr;
+  float* scales = reinterpret_cast<float*>(rows + ((a.P * row_bytes + 255) & ~int64_t(255)));
   const int64_t units = a.P * ((row_bytes + kGatherPiece - 1) / kGatherPiece);
   const int64_t ctas = (units + kGatherThreads / 32 - 1) / (kGatherThreads / 32);
   if (ctas > 0x7FFFFFFF) return cudaErrorInvalidValue;
@@ -474,6 +481,7 @@ static cudaError_t gather_rows(GroupedArgs& a, bool e4m3, void* workspace, cudaS
   a.x_scales = scales;
   a.rows = nullptr;
   a.slots = 1;
+  a.gathered = true;
   return e;
 }
 

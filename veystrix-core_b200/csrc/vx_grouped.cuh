@@ -13,6 +13,13 @@ VX_DEVICE int row_of(const GroupedArgs& a, int p) {
   const int r = __ldg(a.rows + p);
   return r >= 0 && r / a.slots < a.x_rows ? r / a.slots : -1;
 }
+// The scale that a gathered position has if it names no row (a NaN that no
+// other position gets).  Its row is zeros, and so is its output, also where
+// the bank or its scales are no finite numbers.
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+VX_DEVICE bool names_none(const GroupedArgs& a, float scale) {
+  return a.gathered && __float_as_uint(scale) == kNoRow;
+}
 
 // mbar_try that also acquires what the other CTA of the pair released.
 VX_DEVICE bool pair_try(uint32_t bar, uint32_t parity) {
@@ -145,8 +152,9 @@ VX_DEVICE float scaled(float v, float a, float b) {
   return fabsf(p) < 1.f && lo != 0.f ? v * hi * lo : v * lo * hi;
 }
 // Whether v * (a * b) does for every scale a of the warp (N a lane, in s) and
-// every lane's b: no product of theirs that is neither zero nor normal.  One
-// check a tile, so that the tiles' inner loops multiply by the product.
+// every lane's b: no product of theirs that is neither zero nor normal, and no
+// kNoRow.  One check a tile, so that the tiles' inner loops multiply by the
+// product.
 template <int N>
 VX_DEVICE bool products_fit(const float (&s)[N], float b) {
   uint32_t hi = 0, lo = 0x7F800000u;

@@ -94,10 +94,11 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(S)) grouped_few_kernel(c
     }
     // acc: outputs g and g + 8, positions 2 c and 2 c + 1
     auto finish = [&](float v, int n, int pos) {
-      if (FP8) {
-        const int p = p0 + pos, row = a.rows ? row_of(a, p) : p;
-        v = scaled(v, row >= 0 ? __ldg(a.x_scales + row) : 0.f, __ldg(a.w_scales + int64_t(e) * a.N + n));
-      }
+      const int p = p0 + pos, row = a.rows ? row_of(a, p) : p;
+      if (row < 0)
+        v = 0.f;   // names no row: zeros whatever the bank holds
+      else if (FP8)
+        v = scaled(v, __ldg(a.x_scales + row), __ldg(a.w_scales + int64_t(e) * a.N + n));
       a.out[int64_t(p0 + pos) * a.ldo + n] = f32_to_bf16(v);
     };
     if (S == 1) {

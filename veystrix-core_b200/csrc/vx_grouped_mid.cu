@@ -205,6 +205,8 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
       const int rows = c.m() / 4, pos = quarter * rows + lane, n0 = c.n0 + h * (kMidOut / 2);
       const bool real = lane < rows && pos < c.count;
       float sx = 1.f;
+      if ((FP8 || a.gathered) && real) sx = __ldg(a.x_scales + c.p0 + pos);
+      const bool none = names_none(a, sx);
       bool fit = true;
       if (FP8) {
         float sw[4];
@@ -215,7 +217,6 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
           sw[i] = n < a.N ? __ldg(a.w_scales + int64_t(c.e) * a.N + n) : 0.f;
           scale[32 * i + lane] = sw[i];
         }
-        if (real) sx = __ldg(a.x_scales + c.p0 + pos);
         fit = products_fit(sw, sx);
         __syncwarp();
       }
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
           }
           uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = ok ? bf16_pair(v[2 * j], v[2 * j + 1]) : 0x7FFF7FFFu;   // else NaN
+          for (int j = 0; j < 8; ++j) w[j] = !ok ? 0x7FFF7FFFu : none ? 0u : bf16_pair(v[2 * j], v[2 * j + 1]);   // NaN
           if (g.vec == 16 && left >= 16) {
             if (real)
               asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 16 * i), "r"(w[0]),

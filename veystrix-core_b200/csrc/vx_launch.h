@@ -386,6 +386,7 @@ struct GroupedArgs {
   int64_t P;
   uint16_t* out;                // [P][ldo]
   int64_t ldo;
+  bool gathered = false;        // gather_rows has put x in the positions' order; x_scales is its (bf16 too)
 };
 int64_t grouped_workspace_bytes(int64_t P, int experts, int K, bool e4m3, bool rows);   // 0: none
 cudaError_t launch_grouped(GroupedArgs a, bool e4m3, void* workspace, cudaStream_t st);
