@@ -809,8 +809,18 @@ def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape: tup
 
 
 def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
+    """Ids as int32 on dev.  Wider ones are brought to the ends of int32, where
+    they name as little as before."""
     if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
+    if isinstance(t, np.ndarray) and t.dtype.kind in "iu":
+        if t.dtype.kind == "u":
+            t = np.minimum(t.astype(np.uint64), np.uint64(2**31 - 1))
+        t = torch.from_numpy(t.astype(np.int64))
+    elif not isinstance(t, (torch.Tensor, np.ndarray)):
+        t = torch.as_tensor(t)
+    if isinstance(t, torch.Tensor) and t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(-2**31, 2**31 - 1)
     return _i32(t, dev, name)
 
 
