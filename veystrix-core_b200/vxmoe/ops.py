@@ -825,9 +825,14 @@ def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
 
 
 # What a call needs each time, without the Python layers of torch.cuda: the
-# small operators below are host-bound.
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# small operators below are host-bound.  Looked up in the call: a torch built
+# without CUDA has neither, and the package imports with it.
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class AddNorm(NamedTuple):
