@@ -825,14 +825,10 @@ def _ids(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
 
 
 # What a call needs each time, without the Python layers of torch.cuda: the
-# small operators below are host-bound.  Looked up in the call: a torch built
-# without CUDA has neither, and the package imports with it.
-def _current_device() -> int:
-    return torch._C._cuda_getDevice()
-
-
-def _raw_stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+# small operators below are host-bound.  A torch built without CUDA has
+# neither, nor a CUDA tensor that would reach the calls.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class AddNorm(NamedTuple):
