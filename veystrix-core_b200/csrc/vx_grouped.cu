@@ -206,6 +206,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   auto stage_w = [&](int s) { return base + s * kGtStage; };
   auto stage_x = [&](int s) { return base + s * kGtStage + kGtHalf; };
 
+  int stopped_at = 0;               // stage and phase after warp 0's last copies
+  uint32_t stopped_phase = 1;
   if (warp == 0) {
     // ---- copies
     int s = 0;
@@ -237,13 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
         if (++s == kGtStages) s = 0, ph ^= 1;
       }
     }
-    if (dead && rank == 0 && lane == 0) {
-      // given up: let the copies in flight land (bounded)
-      const uint64_t t0 = global_ns();
-      for (int i = 0; i < kGtStages; ++i)
-        while (!mbar_try(smem_u32(&full[i]), i < s ? ph ^ 1 : ph) && global_ns() - t0 < kWaitLimitNs) {
-        }
-    }
+    stopped_at = s, stopped_phase = ph;
   } else if (warp == 1 && rank == 0) {
     // ---- MMAs of the pair: the whole warp waits, one lane issues
     int s = 0, b = 0;
@@ -252,10 +248,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
     int half = pair < tiles ? tile_at(pair).half() : 0;
     for (int t = pair; ok && t < tiles; t += pairs) {
       const uint32_t idesc = uniform(pair_idesc<FP8>(2 * half)), d = tmem + b * kGtCols;
-      ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&acc_empty[b]), aph, &dead));
+      ok = role_wait(smem_u32(&acc_empty[b]), aph, &dead);
       tc_fence_after();
       for (int k = 0; ok && k < steps; ++k) {
-        ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&full[s]), ph, &dead));
+        ok = role_wait(smem_u32(&full[s]), ph, &dead);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -311,7 +307,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
       }
       fetch(t + pairs);
       if (ok) ok = role_wait(smem_u32(&acc_full[b]), ph, &dead);
-      ok = __all_sync(0xFFFFFFFFu, ok);
       tc_fence_after();
       const uint32_t acc = tmem + lanes + b * kGtCols + h * c.half();
       // lane 4 i + q stores column c0 + 4 j + q of outputs 4 i .. 4 i + 3
@@ -367,6 +362,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGtThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (dead && rank == 0 && threadIdx.x == 0) {
+    // given up: let the copies in flight land (bounded)
+    const uint64_t t0 = global_ns();
+    for (int i = 0; i < kGtStages; ++i)
+      while (!mbar_try(smem_u32(&full[i]), i < stopped_at ? stopped_phase ^ 1 : stopped_phase) &&
+             global_ns() - t0 < kWaitLimitNs) {
+      }
+  }
   cluster_sync();   // the peer's copies and MMAs touch this CTA no more
   if (warp == 2) {
     tc_fence_after();

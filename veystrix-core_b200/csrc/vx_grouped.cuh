@@ -36,16 +36,21 @@ VX_DEVICE uint32_t bf16_pair(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Bounded wait of a role: false once this CTA has given up.
+// Bounded wait of a role, by a whole warp: false, in every lane, once this CTA
+// has given up.  (With an answer of its own a lane could leave a loop whose
+// other lanes wait for it at a __syncwarp.)
 VX_DEVICE bool role_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  if (pair_try(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (uint32_t i = 0; i < kSpinLimit; ++i) {
-    if (pair_try(bar, parity)) return true;
-    if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
+  bool done = pair_try(bar, parity);
+  if (!done) {
+    const uint64_t t0 = global_ns();
+    for (uint32_t i = 0; i < kSpinLimit && !done; ++i) {
+      done = pair_try(bar, parity);
+      if ((i & 255) == 255 && (*dead || global_ns() - t0 > kWaitLimitNs)) break;
+    }
   }
-  *dead = 1;
-  return false;
+  done = __all_sync(0xFFFFFFFFu, done);
+  if (!done) *dead = 1;
+  return done;
 }
 
 // Starts of the groups, clamped to [0, P] and to ascend (group e is starts[e]

@@ -124,6 +124,8 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
   auto stage_w = [&](int s) { return base + s * kMidStage; };
   auto stage_x = [&](int s) { return base + s * kMidStage + kMidBank; };
 
+  int stopped_at = 0;               // stage and phase after warp 0's last copies
+  uint32_t stopped_phase = 1;
   if (warp == 0) {
     // ---- copies
     int s = 0;
@@ -153,13 +155,7 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
         if (++s == kMidStages) s = 0, ph ^= 1;
       }
     }
-    if (dead && lane == 0) {
-      // given up: let the copies in flight land (bounded)
-      const uint64_t t0 = global_ns();
-      for (int i = 0; i < kMidStages; ++i)
-        while (!mbar_try(smem_u32(&full[i]), i < s ? ph ^ 1 : ph) && global_ns() - t0 < kWaitLimitNs) {
-        }
-    }
+    stopped_at = s, stopped_phase = ph;
   } else if (warp == 1) {
     // ---- MMAs: the whole warp waits, one lane issues
     int s = 0, b = 0;
@@ -173,10 +169,10 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
       // format 1, e4m3 format 0 of kind::f8f6f4
       const uint32_t f = FP8 ? 0u : 1u;
       const uint32_t idesc = uniform((1u << 4) | (f << 7) | (f << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(c.m() >> 4) << 24));
-      ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&acc_empty[b]), aph, &dead));
+      ok = role_wait(smem_u32(&acc_empty[b]), aph, &dead);
       tc_fence_after();
       for (int k = 0; ok && k < steps; ++k) {
-        ok = __all_sync(0xFFFFFFFFu, role_wait(smem_u32(&full[s]), ph, &dead));
+        ok = role_wait(smem_u32(&full[s]), ph, &dead);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -221,7 +217,6 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
         __syncwarp();
       }
       if (ok) ok = role_wait(smem_u32(&acc_full[b]), ph, &dead);
-      ok = __all_sync(0xFFFFFFFFu, ok);
       tc_fence_after();
       if (quarter * rows < c.count) {   // else no real position in this warp's lanes
         uint16_t* out = a.out + int64_t(c.p0 + pos) * a.ldo + n0;
@@ -293,6 +288,14 @@ __global__ void __launch_bounds__(kMidThreads, 1) grouped_mid_kernel(const __gri
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (dead && threadIdx.x == 0) {
+    // given up: let the copies in flight land (bounded)
+    const uint64_t t0 = global_ns();
+    for (int i = 0; i < kMidStages; ++i)
+      while (!mbar_try(smem_u32(&full[i]), i < stopped_at ? stopped_phase ^ 1 : stopped_phase) &&
+             global_ns() - t0 < kWaitLimitNs) {
+      }
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
