@@ -1,4 +1,4 @@
-"""Source checks of the bounded waits in the grouped kernels.  A wait that ran
+"""Source checks of the bounded waits in the grouped and adapter kernels.  A wait that ran
 out cannot be had on a GPU without stopping one, so what it relies on is read:
 the lanes of a role agree on the outcome, polling ends, and copies in flight
 are awaited once every role of the CTA has stopped."""
@@ -52,3 +52,10 @@ def test_polling_loops_have_a_limit(name):
         assert "kWaitLimitNs" in text[m.start():m.start() + 300]
     for m in re.finditer(r"for \([^;]*; i < kSpinLimit", text):
         assert "kWaitLimitNs" in text[m.start():m.start() + 600]
+
+
+def test_adapter_parts_on_their_way_are_awaited_before_the_cta_leaves():
+    """Peers store into this CTA's shared memory: one that gave up stays for them."""
+    text = source("vx_lora.cu")
+    kernel = body(text, r"lora_small_kernel\(const LoraArgs a\)")
+    assert re.search(r"const bool ok = lora_wait\(&arrived\);\s*if \(!ok\) lora_wait\(&arrived\);", kernel)

@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_small_kernel(const LoraA
   }
   if (rank > 0) {
     const bool ok = lora_wait(&arrived);
+    if (!ok) lora_wait(&arrived);   // given up: let the parts on their way land (bounded)
     const int cols = (rank + 31) & ~31;
     const float scale = ok ? a.scales ? __ldg(a.scales + e) : 1.0f : __uint_as_float(0x7FC00000u);
     uint16_t* f = reinterpret_cast<uint16_t*>(frag);
