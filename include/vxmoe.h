@@ -345,7 +345,8 @@ int vx_rmsnorm(const uint16_t* x, const uint16_t* gain, int32_t T, int32_t d,
  * q * scale; scale = max(max|v| / 448, 2^-126).  A row with a NaN has a NaN
  * scale.  The reference serves bf16 activations over 4-bit banks only; these
  * entry points serve the same layer over bf16 or 8-bit banks.  Widths (d,
- * width, N, K) are at most 2^29, vx_lora_add's N at most 33,553,920. */
+ * width, N) are at most 2^29, vx_lora_add's N at most 33,553,920, K at most
+ * 2^24. */
 #define VX_DTYPE_E4M3 2
 
 /* RMSNorm of s = x + residual (residual NULL: of x): y = bf16(s *

@@ -62,6 +62,10 @@ struct Carver {
 // Widths up to which the row, grouped and adapter kernels' 32-bit column
 // arithmetic holds.
 constexpr int kMaxWidth = 1 << 29;
+// Inputs of a product: a tile over all of them (a third of a microsecond per
+// 128 bytes of a row) and a part of an adapter's inner values stay far below
+// the second after which a wait for them gives up.
+constexpr int kMaxInputs = 1 << 24;
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -1126,7 +1130,7 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
   if (dtype != VX_DTYPE_BF16 && dtype != VX_DTYPE_E4M3) return VX_EINVAL_DTYPE;
   const int size = dtype == VX_DTYPE_BF16 ? 2 : 1;
   if (experts < 1 || experts > kGroupedMaxExperts || N < 1 || K < 1 || slots < 1 || N > kMaxWidth ||
-      K > kMaxWidth)
+      K > kMaxInputs)
     return VX_EINVAL_SHAPE;
   // position numbers, with a tile's padding, stay within 32 bits
   if (P < 0 || P > 0x7FFF0000 || x_rows < 0 || x_rows > 0x7FFF0000 || ldo < N) return VX_EINVAL_SHAPE;
@@ -1152,7 +1156,7 @@ int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, 
                 const int32_t* adapters, const float* scales, const int32_t* ranks, int32_t L, int64_t T, int32_t K,
                 int32_t N, int32_t R, uint16_t* out, int64_t ldo, void* workspace, size_t workspace_bytes,
                 void* stream) {
-  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || K < 8 || K % 8 || K > kMaxWidth || N < 1 ||
+  if (T < 0 || T > 0x7FFF0000 || L < 1 || L > kLoraMaxAdapters || K < 8 || K % 8 || K > kMaxInputs || N < 1 ||
       N > kLoraMaxOut || R < 8 || R % 8 || R > kLoraMaxRank)
     return VX_EINVAL_SHAPE;
   if (ldy < N || ldo < N || ldx < K || ldx % 8) return VX_EINVAL_SHAPE;

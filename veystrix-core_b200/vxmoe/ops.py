@@ -936,8 +936,9 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     bf16 [P, N], P the length of ``rows`` (or M); positions from
     ``offsets[E]`` on are left as they were in ``out`` (undefined when it is
     allocated here), and ``out`` overlaps no input.  K must be a multiple of 16
-    bytes, E at most 2048.  The same call gives the same bits; another number of rows may take another
-    kernel, whose float32 sums run in another order."""
+    bytes and at most 2^24, E at most 2048.  The same call gives the same bits;
+    another number of rows may take another kernel, whose float32 sums run in
+    another order."""
     e4m3 = isinstance(x, torch.Tensor) and x.dtype is torch.float8_e4m3fn
     if not e4m3 and not (isinstance(x, torch.Tensor) and x.dtype is torch.bfloat16):
         raise TypeError("x must be a bfloat16 or float8_e4m3fn tensor")
@@ -1010,9 +1011,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     gets ``y + scales[e] * b[e] @ (a[e] @ x)``, a token whose adapter is
     outside [0, L) (-1: none) gets y.  a [L, R, K] and b [L, N, R] bf16;
     ``scales`` float32 [L]; ``ranks`` int32 [L]: only the first ranks[e] of
-    the R components count.  ``out`` may be y itself and
-    overlaps nothing else.  K and R are multiples of 8, R at most 256, L at
-    most 4096."""
+    the R components count.  ``out`` may be y itself and overlaps nothing else.
+    K and R are multiples of 8, K at most 2^24, R at most 256, L at most 4096."""
     x2, ldx = _row_view(x, "x", torch.bfloat16, align=16)
     y2, ldy = _row_view(y, "y", torch.bfloat16)
     T, K = x2.shape
