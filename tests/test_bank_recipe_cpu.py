@@ -17,7 +17,7 @@ GUIDE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 def test_recipe(dtype):
     with open(GUIDE) as f:
         text = f.read()
-    block = re.search(r"is quantised once at load.*?```python\n(.*?)```", text, re.S).group(1)
+    block = re.search(r"is quantised once at load(?:(?!```|\n#).)*```python\n(.*?)```", text, re.S).group(1)
     w = (torch.randn((3, 5, 32), generator=torch.Generator().manual_seed(1)) * 0.05).to(dtype)
     w[1, 2] = 0
     w[2, 4] = torch.finfo(dtype).smallest_normal

@@ -224,9 +224,11 @@ VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, int r_first, int 
   }
 }
 
-// v = hi + lo in bf16 (lo zero where hi is no finite number).
+// v = hi + lo in bf16 (lo zero where v is no finite number).  A finite v that
+// would round to an infinity takes the largest bf16 as hi.
 VX_DEVICE void lora_split(float v, uint16_t* hi, uint16_t* lo) {
   *hi = f32_to_bf16(v);
+  if ((*hi & 0x7FFFu) == 0x7F80u && fabsf(v) <= 0x1.fffffep127f) *hi -= 1;
   *lo = (*hi & 0x7F80u) != 0x7F80u ? f32_to_bf16(v - bf16_to_f32(*hi)) : uint16_t(0);
 }
 // Place of h's component r of item row `row` in the fragments [16 components]
