@@ -374,10 +374,11 @@ int vx_swiglu_e4m3(const uint16_t* gate, int64_t ldg, const uint16_t* up, int64_
  * both.  Sums in float32, out bf16.  rows and slots fit vx_permute's order
  * over T * slots routed ids: a position reads its token's row of x.
  * Positions from offsets[experts] on are left as they were, and out overlaps
- * no input; a position whose row lies outside [0, x_rows) gets zeros; offsets
- * are clamped to [0, P] and to ascend.  At most 2048 experts; K and ldx are multiples of 16
- * bytes, x and w start on 16-byte boundaries.  The workspace (16-byte aligned) is needed for
- * larger batches with rows (vx_grouped_matmul_workspace is 0 else). */
+ * no input; a position whose row lies outside [0, x_rows) gets zeros, whatever
+ * the bank holds; offsets are clamped to [0, P] and to ascend.  At most 2048
+ * experts; K and ldx are multiples of 16 bytes, x and w start on 16-byte
+ * boundaries.  The workspace (16-byte aligned) is needed for larger batches
+ * with rows (vx_grouped_matmul_workspace is 0 else). */
 size_t vx_grouped_matmul_workspace(int32_t dtype, int64_t P, int32_t experts, int32_t K, int32_t with_rows);
 int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx, const void* w,
                       const float* x_scales, const float* w_scales, const int32_t* offsets,
@@ -390,12 +391,14 @@ int vx_grouped_matmul(const void* x, int32_t dtype, int64_t x_rows, int64_t ldx,
  * adapters[t] (device int32 [T]), a [L, R, K], b [L, N, R] bf16, of which the
  * first ranks[e] (clamped to 0..R) of the R components count; scales and
  * ranks may be NULL (1 and R).  A token whose adapter is outside [0, L) gets
- * y.  Sums in float32, one rounding.  out may be y itself (ldo == ldy) and overlaps nothing
- * else.  K
- * and R are multiples of 8, R <= 256, L <= 4096; x, a and b start on
- * 16-byte boundaries, as do the rows of x.  The workspace (16-byte aligned)
- * is needed above VX_LORA_SMALL tokens (vx_lora_add_workspace is 0 up to
- * there). */
+ * y.  Sums in float32, one rounding; the inner values enter the second product
+ * as two bf16 terms (2^-17), so an output that an infinite b enters is an
+ * infinity or NaN.  The same call gives the same bits; another number of
+ * tokens may sum in another order.  out may be y itself (ldo == ldy) and
+ * overlaps nothing else.  K and R are multiples of 8, R <= 256, L <= 4096; x,
+ * a and b start on 16-byte boundaries, as do the rows of x.  The workspace
+ * (16-byte aligned) is needed above VX_LORA_SMALL tokens
+ * (vx_lora_add_workspace is 0 up to there). */
 #define VX_LORA_SMALL 256
 size_t vx_lora_add_workspace(int64_t T, int32_t L, int32_t R);
 int vx_lora_add(const uint16_t* y, int64_t ldy, const uint16_t* x, int64_t ldx, const uint16_t* a,

@@ -1012,7 +1012,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     outside [0, L) (-1: none) gets y.  a [L, R, K] and b [L, N, R] bf16;
     ``scales`` float32 [L]; ``ranks`` int32 [L]: only the first ranks[e] of
     the R components count.  ``out`` may be y itself and overlaps nothing else.
-    K and R are multiples of 8, K at most 2^24, R at most 256, L at most 4096."""
+    The same call gives the same bits, whatever the other tokens hold; another
+    number of tokens may sum in another order.  The inner values ``a[e] @ x``
+    enter the second product as two bf16 terms: an output that an infinite b
+    enters is an infinity or NaN.  K and R are multiples of 8, K at most 2^24, R at most 256, L at most 4096."""
     x2, ldx = _row_view(x, "x", torch.bfloat16, align=16)
     y2, ldy = _row_view(y, "y", torch.bfloat16)
     T, K = x2.shape
