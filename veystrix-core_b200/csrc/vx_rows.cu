@@ -64,8 +64,8 @@ VX_DEVICE float swiglu_f32(float g, float u) {
   float h, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(g) * -0.72134752f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(h, h, 1.0f)));
-  const float f = g < 0.f ? h : 1.0f;
-  return g * f * r * (u * f);
+  if (g < 0.f) g *= h, u *= h;
+  return g * r * u;
 }
 // The larger of top and |v|, NaN if one of them is.
 VX_DEVICE float max_abs(float top, float v) {
