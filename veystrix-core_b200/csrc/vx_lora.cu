@@ -134,9 +134,10 @@ VX_DEVICE int lora_rank(const LoraArgs& a, int e) {
 
 // A_e x of the item's n tokens over the 32-input blocks first, first + stride,
 // ... of the CTA's warps, 8 * NT components at a time, those from r_first,
-// r_first + r_step, ...; out(row, r, v) gets four neighbouring sums of the CTA.  part: the warps' sums, 128 MT NT floats
-// each.  AHEAD: the next block's operands are loaded before the present one's
-// MMAs.  ready() is called by every thread once, before the first out().
+// r_first + r_step, ...; out(row, r, v) gets four neighbouring sums of the CTA.
+// part: the warps' sums, 128 MT NT floats each.  AHEAD: the next block's
+// operands are loaded before the present one's MMAs.  ready() is called by
+// every thread once, before the first out().
 template <int MT, int NT, bool AHEAD, typename G, typename F>
 VX_DEVICE void lora_shrink(const LoraArgs& a, int e, int rank, int r_first, int r_step, const int* tok, int n,
                            int first, int stride, float* part, G&& ready, F&& out) {
@@ -252,7 +253,8 @@ VX_DEVICE void load_b(const LoraArgs& a, const uint16_t* B, int rank, int nb, in
   for (int u = 0; u < KB; ++u) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = nb * 32 + (WIDE ? 8 * (g >> 1) + 2 * j + (g & 1) : 8 * j + 4 * (g & 1) + (g >> 1)), r = (kb0 + u) * 32 + 8 * c;
+      const int row = nb * 32 + (WIDE ? 8 * (g >> 1) + 2 * j + (g & 1) : 8 * j + 4 * (g & 1) + (g >> 1));
+      const int r = (kb0 + u) * 32 + 8 * c;
       bf[u][j] = r < rank && row < a.N ? __ldg(reinterpret_cast<const uint4*>(B + int64_t(row) * a.R + r))
                                        : make_uint4(0, 0, 0, 0);
     }

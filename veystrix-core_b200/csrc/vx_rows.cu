@@ -37,7 +37,10 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kScaleMin = 0x1p-126f;
 constexpr float kFloatMax = 0x1.fffffep127f;
 
-// {scale, 1/scale} of a row whose largest |v| is amax (NaN stays NaN).
+// {scale, 1/scale} of a row whose largest |v| is amax (NaN stays NaN).  Values
+// are multiplied by the rounded inverse (2^-24 off) rather than divided: one
+// that lies so close to a border between two e4m3 values (whose half step is
+// 2^-4) may go to either.
 VX_DEVICE float2 row_scale(float amax) {
   float s = __fdiv_rn(amax, kE4m3Max);
   s = s < kScaleMin ? kScaleMin : s;
@@ -504,7 +507,7 @@ static cudaError_t per_row_shape(int v, int64_t rows, int width, F&& f) {
     return VX_ROWS(8, 1, false, true);
   }
   // The same with narrower accesses: a warp up to 32 of them a lane, then more
-  // a thread.  Norm 20,000 x 555 36 against 50 us, 13,012 x 1,187 51 / 68, 8,192 x
+  // a thread.  Norm 20,000 x 555 36 against 50 us, 13,012 x 1,187 54 / 68, 8,192 x
   // 1,004 15.2 / 14.7; swiglu 47,605 x 413 25 / 52, 20,000 x 777 21 / 42, 20,000 x
   // 996 17 / 21, 4,000 x 4,002 21 / 25.
   if (v == 4 && many && vecs > 128 && vecs <= 256) return VX_ROWS(4, 8, true, false);

@@ -846,7 +846,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], gain: torch.
     The norm sees the float32 sum before its rounding to the residual's
     type.  ``output``: "bf16" (``y``), "e4m3" (``q`` with one float32 scale a
     row, standing for ``q * scale``), or "both" of the same unrounded values.
-    Where ``rms_norm`` is followed by an 8-bit product this saves the
+    The same call gives the same bits; another number of rows may sum a row in
+    another order.  Where ``rms_norm`` is followed by an 8-bit product this saves the
     separate addition and quantisation passes."""
     if output not in ("bf16", "e4m3", "both"):
         raise ValueError(f"output must be 'bf16', 'e4m3' or 'both', got {output!r}")
